@@ -3,7 +3,8 @@
     python cpu-attention_b200/build.py [--force] [--verbose]
 
 One nvcc process per translation unit, in parallel: csrc/ca_abi.cu (the C ABI,
-the store and prefill kernels), csrc/decode_bf16.cu and csrc/decode_f32.cu (the
+the store and prefill kernels), csrc/ca_serving.cu (8-bit caches, block moves),
+csrc/split_decode.cu (decode over 8-bit caches and windows), csrc/decode_bf16.cu and csrc/decode_f32.cu (the
 decode kernel's instantiations) and csrc/ca_noalloc.cu (the allocation-free
 decode entry), objects under cpu-attention_b200/_build/, linked into
 cpu_attention/libca_b200.so; sm_100a only, with line info, static CUDA runtime. Rebuilds only when a source or this script is newer than the
@@ -47,7 +48,7 @@ def stale():
     return any(os.path.getmtime(f) > t for f in sources())
 
 
-UNITS = ["ca_abi.cu", "ca_noalloc.cu", "decode_bf16.cu", "decode_f32.cu"]
+UNITS = ["ca_abi.cu", "ca_noalloc.cu", "ca_serving.cu", "decode_bf16.cu", "decode_f32.cu", "split_decode.cu"]
 
 
 def build(force=False, verbose=False):

@@ -9,7 +9,7 @@ hand-written CUDA in ``libca_b200.so`` behind a C ABI
 (``include/cpu_attention_b200.h``); tensors are CUDA tensors.
 """
 
-from .cache import reshape_and_cache
+from .cache import append_quantized, compact_blocks, copy_blocks, reshape_and_cache
 from .flash_attn_interface import (
     flash_attn_func,
     flash_attn_kvpacked_func,
@@ -22,6 +22,8 @@ from .flash_attn_interface import (
 
 __version__ = "0.1.0"
 
+# The reference's names (`import *` stays a drop-in). Beyond them the package has
+# append_quantized, copy_blocks and compact_blocks.
 __all__ = [
     "__version__",
     "flash_attn_func",

@@ -22,6 +22,8 @@ import torch
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # `_kernel.py:17`
 HEAD_DIMS = (32, 64, 128)  # `_kernel.py:18`
+EIGHT_BIT = torch.float8_e4m3fn  # the type of caches held in 8 bits
+EIGHT_BIT_CODE = 2
 _DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libca_b200.so"
 
@@ -49,6 +51,17 @@ SIGNATURES = {
                                  _I64, _I64, _I64, _I64, _I32, _F, _P]),
     "ca_flash": (_I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _PI64, _PI64, _PI64, _F, _I32, _I32, _P,
                         _P]),
+    "ca_flash_window": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _PI64, _PI64, _PI64, _P, _P,
+                               _I64, _I64, _F, _I32, _I64, _I64, _I64, _I32, _P, _P]),
+    "ca_append_8bit": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64,
+                              _I64, _I64, _I32, _P, _P]),
+    "ca_decode_split_workspace_bytes": (_SZ, [_I64, _I32]),
+    "ca_decode_split": (_I32, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64,
+                               _I64, _I64, _I64, _I64, _I32, _I32, _I64, _I64, _F, _P, _SZ, _P, _P]),
+    "ca_copy_blocks": (_I32, [_P, _PI64, _I64, _I64, _P, _I64, _P, _P]),
+    "ca_compact_workspace_bytes": (_SZ, [_I64]),
+    "ca_compact_blocks": (_I32, [_P, _PI64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ, _P,
+                                 _P]),
     "ca_status": (_I32, [_P, _I32, _P]),
     "ca_set_wait_limit_ns": (None, [ctypes.c_uint64]),
     "ca_last_cuda_error": (ctypes.c_char_p, []),

@@ -4,8 +4,10 @@ Names, parameters, defaults and exception texts are the reference's
 (`cpu_attention/flash_attn_interface.py`), so code written for it runs
 unchanged. Beyond the reference, this build attends grouped heads (GQA/MQA:
 ``nheads_k`` divides ``nheads``), returns the softmax log-sum-exp
-(``return_softmax_lse`` here, ``return_attn_probs`` for prefill) and runs
-``flash_attn_varlen_func``.
+(``return_softmax_lse`` here, ``return_attn_probs`` for prefill), runs
+``flash_attn_varlen_func``, attends caches held in 8 bits (``k_descale`` /
+``v_descale``) and attends behind a sliding window whose first tokens stay
+visible (``window_size`` with ``sink_tokens``).
 
 A call goes to the native entry (``_native``) with its arguments as given. The
 native entry answers None when it cannot use them; only then does this module
@@ -19,11 +21,11 @@ import torch
 
 from . import _kernel as K
 from . import _native
-from .cache import reshape_and_cache
+from .cache import check_eight_bit, reshape_and_cache
 
 # flash_attn_with_kvcache options no kernel here implements; setting one raises
-_NOT_SUPPORTED = ("cpu_attention: qv, rotary, cache_leftpad, varlen, descale, sliding windows, softcap, "
-                  "attention_chunk and alibi are not supported")
+_NOT_SUPPORTED = ("cpu_attention: qv, rotary, cache_leftpad, varlen, descale of float caches, sliding windows without "
+                  "sink_tokens, softcap, attention_chunk and alibi are not supported")
 
 
 def _as_tensor(x):
@@ -90,6 +92,7 @@ def flash_attn_with_kvcache(
     return_softmax_lse=False,
     block_table=None,
     alibi_slopes=None,
+    sink_tokens=None,
 ):
     """One query token per sequence attending its paged K/V cache.
 
@@ -106,18 +109,35 @@ def flash_attn_with_kvcache(
     sits at the last cached position, so ``causal`` changes nothing; the
     scheduling hints (``num_splits``, ``pack_gqa``, ...) are not needed. The
     other flash-attn options raise ``NotImplementedError``.
+
+    Caches held in 8 bits (``torch.float8_e4m3fn``, written by
+    ``append_quantized`` or ``k``/``v`` here, both sides ``[num_blocks,
+    nheads_k, page_block_size, headdim]`` without a transpose) come with
+    ``k_descale`` and ``v_descale``, float32 ``[num_blocks, nheads_k]``: a value
+    is its code times its block's and head's scale. ``q`` (and ``k``/``v``) stay
+    fp32 or bf16; appending updates caches and scales.
+
+    ``sink_tokens`` (0 or more) turns ``window_size`` on, for float and 8-bit
+    caches: the query, at the last position, sees the last ``window_size[0] +
+    1`` tokens and the first ``sink_tokens`` ones (``window_size[0] = -1``: all).
+    Pages wholly between the two are never read; their page-table entries may
+    be anything (``compact_blocks`` frees them). Without ``sink_tokens`` a
+    window is refused, as in the reference.
     """
     # (every option at its default: the common case, decided without building
     # the option table -- an engine calls this once per layer and token)
     if not (qv is None and rotary_cos is None and rotary_sin is None and cache_leftpad is None
             and cu_seqlens_q is None and cu_seqlens_k_new is None and max_seqlen_q is None
             and rotary_seqlens is None and q_descale is None and k_descale is None and v_descale is None
-            and alibi_slopes is None and not attention_chunk and not softcap and window_size == (-1, -1)) \
+            and alibi_slopes is None and sink_tokens is None and not attention_chunk and not softcap
+            and window_size == (-1, -1)) \
             and _options_set(dict(qv=qv, rotary_cos=rotary_cos, rotary_sin=rotary_sin, cache_leftpad=cache_leftpad,
                                   cu_seqlens_q=cu_seqlens_q, cu_seqlens_k_new=cu_seqlens_k_new,
                                   max_seqlen_q=max_seqlen_q, rotary_seqlens=rotary_seqlens, q_descale=q_descale,
-                                  k_descale=k_descale, v_descale=v_descale, window_size=window_size,
-                                  softcap=softcap, attention_chunk=attention_chunk, alibi_slopes=alibi_slopes)):
+                                  softcap=softcap, attention_chunk=attention_chunk, alibi_slopes=alibi_slopes,
+                                  **({} if k_cache.dtype == K.EIGHT_BIT
+                                     else dict(k_descale=k_descale, v_descale=v_descale)),
+                                  **({} if sink_tokens is not None else dict(window_size=window_size)))):
         raise NotImplementedError(_NOT_SUPPORTED)
     if block_table is not None and page_table is not None:
         raise ValueError("cpu_attention: pass `page_table` or `block_table`, not both")
@@ -138,6 +158,16 @@ def flash_attn_with_kvcache(
     def finish(out):
         return (out, lse.unsqueeze(-1)) if return_softmax_lse else out
 
+    if sink_tokens is not None or k_cache.dtype == K.EIGHT_BIT:
+        left, _, sinks = _window(window_size, 0 if sink_tokens is None else sink_tokens)
+        args = (q, k_cache, v_cache, k, v, k_descale, v_descale, lens, table)
+        out = _native.decode_split(0, *args, left, sinks, softmax_scale, lse)
+        if out is None:
+            args = _explain_split(*args)
+            out = _native.decode_split(0, *args, left, sinks, softmax_scale, lse)
+            if out is None:
+                raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
+        return finish(out)
     if k is not None and k.shape[1] > 1:
         # a prompt of several new tokens: the decode launch appends them itself
         # when it can read everything in place
@@ -162,6 +192,69 @@ def flash_attn_with_kvcache(
         if out is None:
             raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
     return finish(out)
+
+
+def _window(window_size, sink_tokens):
+    """(left, right, sinks) of a window, checked."""
+    try:
+        left, right = (int(x) for x in window_size)
+        sinks = int(sink_tokens)
+    except (TypeError, ValueError):
+        raise ValueError("cpu_attention: window_size must be two ints and sink_tokens an int") from None
+    if left < -1 or right < -1 or sinks < 0:
+        raise ValueError("cpu_attention: window_size must be (left, right) of -1 or more and sink_tokens 0 or more "
+                         f"(got {tuple(window_size)}, {sink_tokens})")
+    return left, right, min(sinks, 1 << 30)
+
+
+def _explain_split(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table):
+    """Called when the split decode declined: the checks of ``_explain_decode``
+    for 8-bit caches and windows, several new tokens included."""
+    q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table = (
+        _as_tensor(x) for x in (q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table))
+    if q.dim() != 4:
+        raise ValueError("cpu_attention: q must be [batch, 1, nheads, headdim]")
+    if q.shape[1] != 1:
+        raise NotImplementedError("cpu_attention decodes one query token per sequence")
+    batch, _, heads, hd = q.shape
+    eight = k_cache.dtype == K.EIGHT_BIT
+    new = 0 if k is None else (k.shape[1] if k.dim() == 4 else -1)
+    if eight:
+        check_eight_bit(k_cache, v_cache, k_scale, v_scale)
+    elif k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("cpu_attention: k_cache/v_cache must be "
+                         "[num_blocks, nheads, page_block_size, headdim] and match")
+    kv_heads = k_cache.shape[1]
+    if k_cache.shape[3] != hd or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError("cpu_attention: q and the caches disagree on heads or head_dim")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("cpu_attention: the paged caches must be contiguous")
+    if q.dtype not in K.DTYPES or (not eight and (k_cache.dtype != q.dtype or v_cache.dtype != q.dtype)):
+        raise ValueError("cpu_attention: q and the caches must share a dtype (fp32 or bf16)")
+    if hd not in K.HEAD_DIMS or k_cache.shape[2] % 16 or k_cache.shape[2] < 1:
+        raise ValueError(f"cpu_attention: head_dim must be 32/64/128 (got {hd}) and the "
+                         f"page a multiple of 16 (got {k_cache.shape[2]})")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch:
+        raise ValueError("cpu_attention: page_table must be int32 [batch, max_blocks]")
+    if table.shape[1] * k_cache.shape[2] > 0x7fffffff:
+        raise ValueError("cpu_attention: page_table must not hold more than 2^31 - 1 positions per sequence")
+    if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,):
+        raise ValueError("cpu_attention: cache_seqlens must be an int or an int32 [batch] tensor")
+    if (k is None) != (v is None) or k is not None and (
+            new < 0 or tuple(k.shape) != (batch, new, kv_heads, hd) or v.shape != k.shape or k.dtype != q.dtype
+            or v.dtype != q.dtype):
+        raise ValueError("cpu_attention: k/v must both be [batch, seqlen_new, nheads, headdim]")
+    if batch and int(lens.max()) + new > table.shape[1] * k_cache.shape[2]:
+        raise ValueError("cpu_attention: cache_seqlens exceed the page table's capacity")
+    dev = q.device
+    data = [k_cache, v_cache] + ([k, v] if k is not None else []) + ([k_scale, v_scale] if eight else [])
+    if dev.type != "cuda" or any(t.device != dev for t in data):
+        raise ValueError("cpu_attention: q, the caches and k/v must be CUDA tensors on one device "
+                         f"(q is on {dev})")
+    if k is not None:
+        k, v = k.contiguous(), v.contiguous()
+    q = q.contiguous()
+    return (q, k_cache, v_cache, k, v, k_scale, v_scale, _to(lens.contiguous(), dev), _to(table.contiguous(), dev))
 
 
 def _explain_decode(q, k_cache, v_cache, k, v, table, lens):
@@ -206,7 +299,8 @@ def _explain_decode(q, k_cache, v_cache, k, v, table, lens):
     return (_readable_rows(q), k_cache, v_cache, k, v, _to(table.contiguous(), dev), _to(lens.contiguous(), dev))
 
 
-def flash_attn_func(q, k, v, softmax_scale=None, causal=False, *, return_attn_probs=False):
+def flash_attn_func(q, k, v, softmax_scale=None, causal=False, *, return_attn_probs=False, window_size=(-1, -1),
+                    sink_tokens=0):
     """Attention over whole sequences (prefill), flash-attn's ``flash_attn_func``.
 
     q ``[batch, seqlen_q, nheads, headdim]``, k/v ``[batch, seqlen_k, nheads_k,
@@ -216,18 +310,35 @@ def flash_attn_func(q, k, v, softmax_scale=None, causal=False, *, return_attn_pr
     seqlen_q``, and a row that sees no key is zero. ``softmax_scale`` defaults
     to ``headdim ** -0.5``. ``return_attn_probs`` (flash-attn 3's name) also
     returns the float32 ``[batch, nheads, seqlen_q]`` softmax log-sum-exp.
-    Inference only: no dropout, window, softcap or alibi.
+    Inference only: no dropout, softcap or alibi.
+
+    ``window_size=(left, right)`` (-1: no limit, the default) hides keys more
+    than ``left`` before or ``right`` after a row's position ``i + seqlen_k -
+    seqlen_q`` (``causal``: right is 0), but the first ``sink_tokens`` keys stay
+    visible behind the window. Key tiles that no row of a query tile sees are
+    not read; in tiles that are, values (also those of hidden keys) have to be
+    finite.
     """
+    window = _prefill_window(window_size, sink_tokens)
     lse = None
     if return_attn_probs and q.dim() == 4:
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-    out = _native.flash(0, q, k, v, softmax_scale, causal, lse)
+    out = _native.flash(0, q, k, v, softmax_scale, causal, lse, window=window)
     if out is None:
         q, k, v = _explain_flash(q, k, v)
-        out = _native.flash(0, q, k, v, softmax_scale, bool(causal), lse)
+        out = _native.flash(0, q, k, v, softmax_scale, bool(causal), lse, window=window)
         if out is None:
             raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
     return (out, lse) if return_attn_probs else out
+
+
+def _prefill_window(window_size, sink_tokens):
+    """The window given to the prefill entries, or None when it hides nothing
+    (sinks alone change nothing)."""
+    if sink_tokens == 0 and window_size == (-1, -1):
+        return None
+    window = _window(window_size, sink_tokens)
+    return None if window[:2] == (-1, -1) else window
 
 
 def _explain_flash(q, k, v):
@@ -255,7 +366,7 @@ def _check_dtypes_and_device(q, k, v, hd):
 
 
 def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale=None,
-                           causal=False, *, return_attn_probs=False):
+                           causal=False, *, return_attn_probs=False, window_size=(-1, -1), sink_tokens=0):
     """``flash_attn_func`` over sequences of different lengths packed end to end.
 
     q is ``[total_q, nheads, headdim]`` and k/v ``[total_k, nheads_k, headdim]``;
@@ -264,18 +375,20 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
     starting at 0). ``max_seqlen_q``/``max_seqlen_k`` bound the lengths. The
     causal mask is bottom-right within each sequence. Returns ``[total_q,
     nheads, headdim]``, and with ``return_attn_probs`` also the float32
-    ``[nheads, total_q]`` log-sum-exp.
+    ``[nheads, total_q]`` log-sum-exp. ``window_size`` and ``sink_tokens`` as in
+    ``flash_attn_func``, within each sequence.
     """
+    window = _prefill_window(window_size, sink_tokens)
     lse = None
     if return_attn_probs and q.dim() == 3:
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
     out = _native.flash(0, q, k, v, softmax_scale, causal, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
-                        max_seqlen_k)
+                        max_seqlen_k, window)
     if out is None:
         q, k, v, cu_seqlens_q, cu_seqlens_k = _explain_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
                                                               max_seqlen_k)
         out = _native.flash(0, q, k, v, softmax_scale, bool(causal), lse, cu_seqlens_q, cu_seqlens_k,
-                            int(max_seqlen_q), int(max_seqlen_k))
+                            int(max_seqlen_q), int(max_seqlen_k), window)
         if out is None:
             raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
     return (out, lse) if return_attn_probs else out

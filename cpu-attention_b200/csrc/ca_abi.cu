@@ -3,6 +3,7 @@
 // stream. Declarations and the contract live in include/cpu_attention_b200.h.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdio>
@@ -55,6 +56,23 @@ int current_device(int* dev) {
   cudaError_t e = cudaGetDevice(dev);
   return e == cudaSuccess ? CA_OK : cuda_fail(e, "cudaGetDevice");
 }
+
+}  // namespace
+
+namespace ca {
+int host_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+int host_sms(int* sms) {
+  int device;
+  int rc = current_device(&device);
+  if (rc) return rc;
+  DeviceInfo dev;
+  if ((rc = device_info(device, &dev))) return rc;
+  *sms = dev.sms;
+  return CA_OK;
+}
+}  // namespace ca
+
+namespace {
 
 // ---- decode plan ---------------------------------------------------------
 struct DecodePlan {
@@ -389,6 +407,17 @@ int ca_flash_ex(const void* q, const void* k, const void* v, void* out, float* l
                 const int64_t k_strides[3], const int64_t v_strides[3], const int32_t* cu_seqlens_q,
                 const int32_t* cu_seqlens_k, int64_t total_q, int64_t total_k, float softmax_scale, int causal,
                 int dtype, int32_t* status, void* stream) {
+  return ca_flash_window(q, k, v, out, lse, batch, seq_q, seq_k, heads, kv_heads, head_dim, q_strides, k_strides,
+                         v_strides, cu_seqlens_q, cu_seqlens_k, total_q, total_k, softmax_scale, causal, -1, -1, 0,
+                         dtype, status, stream);
+}
+
+int ca_flash_window(const void* q, const void* k, const void* v, void* out, float* lse, int64_t batch,
+                    int64_t seq_q, int64_t seq_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                    const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t total_q, int64_t total_k,
+                    float softmax_scale, int causal, int64_t window_left, int64_t window_right, int64_t sink_tokens,
+                    int dtype, int32_t* status, void* stream) {
   if (dtype != CA_DTYPE_F32 && dtype != CA_DTYPE_BF16) return CA_EDTYPE;
   if (!head_dim_ok(head_dim)) return CA_EHEADDIM;
   const bool var = cu_seqlens_q != nullptr || cu_seqlens_k != nullptr;
@@ -397,6 +426,7 @@ int ca_flash_ex(const void* q, const void* k, const void* v, void* out, float* l
   if (var && (!cu_seqlens_q || !cu_seqlens_k || total_q < 0 || total_k < 0 || total_q > 0x7fffffffLL ||
               total_k > 0x7fffffffLL))
     return CA_ESHAPE;
+  if (window_left < -1 || window_right < -1 || sink_tokens < 0) return CA_ESHAPE;
   if (batch == 0 || (var && total_q == 0)) return CA_OK;
   if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides) return CA_ENULL;
   const size_t es = elem_size(dtype);
@@ -426,6 +456,12 @@ int ca_flash_ex(const void* q, const void* k, const void* v, void* out, float* l
   prm.total_k = var ? total_k : 0;
   prm.c = (float)(scale * 1.4426950408889634);
   prm.causal = causal ? 1 : 0;
+  // no side of the window can matter past the longest sequence
+  const int64_t most = seq_q > seq_k ? seq_q : seq_k;
+  prm.win = window_left >= 0 || window_right >= 0;
+  prm.left = window_left < 0 ? -1 : (int)std::min(window_left, most);
+  prm.right = causal ? 0 : (window_right < 0 ? -1 : (int)std::min(window_right, most));
+  prm.sinks = prm.win ? (int)std::min(sink_tokens, seq_k) : 0;
   int device;
   int rc = current_device(&device);
   if (rc) return rc;

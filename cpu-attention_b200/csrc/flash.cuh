@@ -32,7 +32,24 @@ struct FlashParams {
   long long total_q, total_k;      // varlen: tokens of q and of k/v (lse is [H, total_q])
   float c;                         // softmax_scale * log2(e)
   int causal;
+  // a sliding window (win != 0; causal is then part of `right`): row i, at
+  // position i + Lk - Lq, sees keys from `left` before it (and the first
+  // `sinks` keys) to `right` after it; a negative side has no limit
+  int win, left, right, sinks;
 };
+
+// The keys row i of a windowed launch sees: j <= hi and (j >= lo or j < sinks).
+struct FlashWindow {
+  int lo, hi;
+};
+template <typename P>
+__device__ __forceinline__ FlashWindow flash_window(const P& p, int i, int Lq, int Lk) {
+  const long long at = (long long)i + Lk - Lq;
+  FlashWindow w;
+  w.lo = p.left < 0 ? 0 : (int)max(0LL, at - p.left);
+  w.hi = p.right < 0 ? Lk - 1 : (int)min((long long)Lk - 1, at + p.right);
+  return w;
+}
 
 // A CTA's sequence of a prefill launch: its lengths, where its tokens start
 // and where its output rows and log-sum-exps go.
@@ -98,7 +115,7 @@ constexpr int RW = 16;  // rows per warp
 constexpr int KP = BK + 1;
 }  // namespace generic
 
-template <typename T, int E>
+template <typename T, int E, bool WIN>
 __global__ void __launch_bounds__(128) flash_generic_kernel(const __grid_constant__ FlashParams p) {
   using namespace generic;
   constexpr int DPL = E / 32;  // output dims per lane
@@ -109,7 +126,7 @@ __global__ void __launch_bounds__(128) flash_generic_kernel(const __grid_constan
   float* sP = sQ + BQ * E;       // [4 warps][BK][RW]  (key-major: 4 rows per float4)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int blk, h, b;
-  flash_block_of((int)blockIdx.x, (p.Lq + BQ - 1) / BQ, p.H, p.causal != 0, &blk, &h, &b);
+  flash_block_of((int)blockIdx.x, (p.Lq + BQ - 1) / BQ, p.H, !WIN && p.causal != 0, &blk, &h, &b);
   const int q0 = blk * BQ;
   const FlashSeq sq = flash_seq(p, b, h, E);
   const int Lq = sq.Lq, Lk = sq.Lk;
@@ -129,7 +146,12 @@ __global__ void __launch_bounds__(128) flash_generic_kernel(const __grid_constan
     sQ[x] = qi < Lq ? to_f32(qg[(long long)qi * p.qs[1] + d]) : 0.f;
   }
 
-  const int kend = p.causal ? min(Lk, q0 + BQ + diag) : Lk;  // keys [0, kend) can be visible
+  int kend = p.causal ? min(Lk, q0 + BQ + diag) : Lk;  // keys [0, kend) can be visible
+  int klo = 0;                                          // and, windowed, from klo on or below p.sinks
+  if constexpr (WIN) {
+    klo = flash_window(p, q0, Lq, Lk).lo;
+    kend = flash_window(p, min(q0 + BQ, Lq) - 1, Lq, Lk).hi + 1;
+  }
   float m[RW], lp[RW], o[RW][DPL];
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -142,6 +164,10 @@ __global__ void __launch_bounds__(128) flash_generic_kernel(const __grid_constan
   float* sPw = sP + warp * BK * RW;
 
   for (int k0 = 0; k0 < kend; k0 += BK) {
+    if constexpr (WIN) {
+      // past the first keys, on to the window's first tile
+      if (k0 >= p.sinks && k0 + BK <= klo) k0 = klo / BK * BK;
+    }
     __syncthreads();  // previous tile consumed (and Q written, first time)
     for (int x = threadIdx.x; x < BK * E; x += blockDim.x) {
       const int j = x / E, d = x - j * E;
@@ -155,7 +181,7 @@ __global__ void __launch_bounds__(128) flash_generic_kernel(const __grid_constan
       sV[j * E + d] = vv;
     }
     __syncthreads();
-    if (p.causal && k0 > wr0 + RW - 1 + diag) continue;  // nothing visible to this warp
+    if (!WIN && p.causal && k0 > wr0 + RW - 1 + diag) continue;  // nothing visible to this warp
 
     // S = Q K^T for 16 rows x keys {lane, lane+32}
     float s0[RW], s1[RW];
@@ -189,8 +215,14 @@ __global__ void __launch_bounds__(128) flash_generic_kernel(const __grid_constan
       const int qi = wr0 + r;
       const int lim = p.causal ? min(Lk - 1, qi + diag) : Lk - 1;  // last visible key
       const int j0 = k0 + lane, j1 = k0 + lane + 32;
-      const float x0 = (j0 <= lim) ? s0[r] * p.c : -INFINITY;
-      const float x1 = (j1 <= lim) ? s1[r] * p.c : -INFINITY;
+      bool on0 = j0 <= lim, on1 = j1 <= lim;
+      if constexpr (WIN) {
+        const FlashWindow w = flash_window(p, qi, Lq, Lk);
+        on0 = j0 <= w.hi && (j0 >= w.lo || j0 < p.sinks);
+        on1 = j1 <= w.hi && (j1 >= w.lo || j1 < p.sinks);
+      }
+      const float x0 = on0 ? s0[r] * p.c : -INFINITY;
+      const float x1 = on1 ? s1[r] * p.c : -INFINITY;
       const float mx = warp_max(fmaxf(x0, x1));
       const float mn = fmaxf(m[r], mx);
       float p0 = 0.f, p1 = 0.f, alpha = 1.f;
@@ -262,15 +294,16 @@ inline cudaError_t smem_limit_once(const void* kern, int smem, unsigned char (&d
 template <typename T, int E>
 int flash_generic_launch(const FlashParams& p, cudaStream_t stream, std::string* err) {
   const size_t smem = flash_generic_smem(E);
-  static unsigned char configured[64] = {0};
-  cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(flash_generic_kernel<T, E>), (int)smem, configured);
+  static unsigned char configured[2][64] = {};
+  auto kern = p.win ? flash_generic_kernel<T, E, true> : flash_generic_kernel<T, E, false>;
+  cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), (int)smem, configured[p.win ? 1 : 0]);
   if (e != cudaSuccess) {
     *err = std::string("cudaFuncSetAttribute(flash): ") + cudaGetErrorString(e);
     return CA_ECUDA;
   }
   const long long ctas = (long long)((p.Lq + generic::BQ - 1) / generic::BQ) * p.H * p.B;
   if (ctas > 0x7fffffffLL) return CA_EUNSUPPORTED;
-  flash_generic_kernel<T, E><<<(unsigned)ctas, 128, smem, stream>>>(p);
+  kern<<<(unsigned)ctas, 128, smem, stream>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) {
     *err = std::string("flash launch: ") + cudaGetErrorString(e);

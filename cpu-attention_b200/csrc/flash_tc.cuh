@@ -48,6 +48,7 @@ struct FlashTcArgs {
   int G;                   // query heads per KV head
   float c;                 // softmax_scale * log2(e)
   int causal;
+  int left, right, sinks;  // windowed launches (see FlashParams)
   int* status;
 };
 
@@ -150,7 +151,21 @@ __device__ __forceinline__ int tc_tiles(int r0, int Lq, int Lk, bool causal) {
   return kend > 0 ? (kend + 127) / 128 : 0;
 }
 
-template <int E, bool CAUSAL>
+// The 128-key tiles a windowed CTA reads: the first keys' tiles [0, ns), then,
+// `skip` tiles later, those from its first row's window on.
+struct TcTiles {
+  int ns, skip;
+  __device__ __forceinline__ int real(int j) const { return j < ns ? j : j + skip; }
+};
+
+// Bits [a, b) of a word (a, b clamped to [0, 32]).
+__device__ __forceinline__ uint32_t bit_range(int a, int b) {
+  const uint32_t below_b = b >= 32 ? 0xffffffffu : (b <= 0 ? 0u : (1u << b) - 1u);
+  const uint32_t below_a = a >= 32 ? 0xffffffffu : (a <= 0 ? 0u : (1u << a) - 1u);
+  return below_b & ~below_a;
+}
+
+template <int E, bool CAUSAL, bool WIN>
 __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant__ FlashTcArgs a) {
   using C = TcCfg<E>;
   extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
@@ -171,7 +186,24 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
   const int kh = h / a.G;                    // the KV head of query head h
   const int tb = a.cu_q ? 0 : b;             // TMA batch coordinate
   const int tq = (int)sq.tq0, tk = (int)sq.tk0;  // TMA token offsets (varlen)
-  const int nt0 = tc_tiles(q0, Lq, Lk, CAUSAL), nt1 = tc_tiles(q0 + C::BM, Lq, Lk, CAUSAL);
+  int nt0 = tc_tiles(q0, Lq, Lk, CAUSAL), nt1 = tc_tiles(q0 + C::BM, Lq, Lk, CAUSAL);
+  TcTiles tiles{0, 0};
+  if constexpr (WIN) {
+    // tiles are numbered without those that no row of the CTA sees (tile B
+    // starts with A's: the rows of B mask what lies before their window). A
+    // row's window ends at or after its start, so a query tile that sees
+    // anything has tiles past the skipped ones.
+    auto count = [&](int r0) {
+      if (r0 >= Lq) return 0;
+      return (max(0, flash_window(a, min(r0 + C::BM, Lq) - 1, Lq, Lk).hi + 1) + C::BN - 1) / C::BN;
+    };
+    nt0 = count(q0);
+    nt1 = count(q0 + C::BM);
+    tiles.ns = (a.sinks + C::BN - 1) / C::BN;
+    tiles.skip = max(0, (q0 < Lq ? flash_window(a, q0, Lq, Lk).lo : 0) / C::BN - tiles.ns);
+    nt0 = max(0, nt0 - tiles.skip);
+    nt1 = max(0, nt1 - tiles.skip);
+  }
   const int nt = max(nt0, nt1);
 
   if (threadIdx.x == 0) {
@@ -219,7 +251,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
         mbar_arrive_expect_tx(&bars->kf[ks], C::TILE_BYTES);
 #pragma unroll
         for (int ch = 0; ch < C::NCH; ++ch)
-          tc::tma_load_4d(sK + ks * C::TILE_BYTES + ch * C::CH_BYTES, &a.tk, ch * C::CHUNK, tk + j * C::BN, kh,
+          tc::tma_load_4d(sK + ks * C::TILE_BYTES + ch * C::CH_BYTES, &a.tk, ch * C::CHUNK, tk + (WIN ? tiles.real(j) : j) * C::BN, kh,
                           tb, &bars->kf[ks]);
         // the V tiles whose slot is free by now
         for (; jv <= j; ++jv) {
@@ -228,7 +260,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
           mbar_arrive_expect_tx(&bars->vf[vs], C::TILE_BYTES);
 #pragma unroll
           for (int ch = 0; ch < C::NCH; ++ch)
-            tc::tma_load_4d(sV + vs * C::TILE_BYTES + ch * C::CH_BYTES, &a.tv, ch * C::CHUNK, tk + jv * C::BN, kh,
+            tc::tma_load_4d(sV + vs * C::TILE_BYTES + ch * C::CH_BYTES, &a.tv, ch * C::CHUNK, tk + (WIN ? tiles.real(jv) : jv) * C::BN, kh,
                             tb, &bars->vf[vs]);
         }
       }
@@ -238,7 +270,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
         mbar_arrive_expect_tx(&bars->vf[vs], C::TILE_BYTES);
 #pragma unroll
         for (int ch = 0; ch < C::NCH; ++ch)
-          tc::tma_load_4d(sV + vs * C::TILE_BYTES + ch * C::CH_BYTES, &a.tv, ch * C::CHUNK, tk + jv * C::BN, kh,
+          tc::tma_load_4d(sV + vs * C::TILE_BYTES + ch * C::CH_BYTES, &a.tv, ch * C::CHUNK, tk + (WIN ? tiles.real(jv) : jv) * C::BN, kh,
                           tb, &bars->vf[vs]);
       }
       // leave only after every load this CTA issued has landed
@@ -308,7 +340,13 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
     const uint32_t lrow = tmem + ((uint32_t)(grp * 32) << 16);
     const uint32_t tS = lrow + C::T_S(x), tO = lrow + C::T_O(x);
     const int qi = q0 + x * C::BM + r;
-    const int lim = CAUSAL ? min(Lk - 1, qi + Lk - Lq) : Lk - 1;  // last key this row sees
+    int lim = CAUSAL ? min(Lk - 1, qi + Lk - Lq) : Lk - 1;  // last key this row sees
+    int low = 0;                                             // windowed: the first past a.sinks
+    if constexpr (WIN) {
+      const FlashWindow w = flash_window(a, qi, Lq, Lk);
+      lim = w.hi;
+      low = w.lo;
+    }
     const int ntr = (x ? nt1 : nt0);
     // masked scores get a value that scale * value maps to -inf
     const float sent = a.c >= 0.f ? -INFINITY : INFINITY;
@@ -334,9 +372,26 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
 #pragma unroll
       for (int c4 = 0; c4 < C::BN / 32; ++c4) tc::tmem_ld32(tS + c4 * 32, *reinterpret_cast<uint32_t(*)[32]>(sr + c4 * 32));
       tc::tmem_ld_wait();
-      const int k0 = j * C::BN;
-      const bool full = (k0 + C::BN - 1) <= lim;
-      if (!full) {
+      const int k0 = (WIN ? tiles.real(j) : j) * C::BN;
+      bool full = (k0 + C::BN - 1) <= lim;
+      // windowed: one bit per key of the tile that this row sees
+      uint32_t seen[WIN ? C::BN / 32 : 1];
+      if constexpr (WIN) {
+        full = full && (k0 >= low || k0 + C::BN <= a.sinks);
+        if (!full) {
+#pragma unroll
+          for (int w = 0; w < C::BN / 32; ++w) {
+            const int at = k0 + 32 * w;
+            seen[w] = bit_range(low - at, lim + 1 - at) | bit_range(0, min(a.sinks, lim + 1) - at);
+          }
+#pragma unroll
+          for (int i = 0; i < C::BN; ++i)
+            if (!((seen[i / 32] >> (i % 32)) & 1u)) sr[i] = __float_as_uint(sent);
+        } else {
+#pragma unroll
+          for (int w = 0; w < C::BN / 32; ++w) seen[w] = 0xffffffffu;
+        }
+      } else if (!full) {
 #pragma unroll
         for (int i = 0; i < C::BN; ++i)
           if (k0 + i > lim) sr[i] = __float_as_uint(sent);
@@ -383,7 +438,10 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
             const int e0 = ch * 32 + 2 * i;
             const uint64_t xe = fma_f32x2(f32x2(__uint_as_float(sr[e0]), __uint_as_float(sr[e0 + 1])), c2v, nm2);
             float p0 = exp2_approx(lo_f32(xe)), p1 = exp2_approx(hi_f32(xe));
-            if constexpr (decltype(masked)::value) {
+            if constexpr (decltype(masked)::value && WIN) {
+              p0 = (seen[e0 / 32] >> (e0 % 32)) & 1u ? p0 : 0.f;
+              p1 = (seen[e0 / 32] >> (e0 % 32 + 1)) & 1u ? p1 : 0.f;
+            } else if constexpr (decltype(masked)::value) {
               p0 = k0 + e0 <= lim ? p0 : 0.f;
               p1 = k0 + e0 + 1 <= lim ? p1 : 0.f;
             }
@@ -531,19 +589,24 @@ int flash_tc_launch(const FlashParams& p, int* status, cudaStream_t stream, std:
   a.G = p.G;
   a.c = p.c;
   a.causal = p.causal;
+  a.left = p.left;
+  a.right = p.right;
+  a.sinks = p.sinks;
   a.status = status;
-  static unsigned char configured[2][64] = {};
-  static int regs_ok[2] = {0, 0};  // 0: not checked, 1: as planned, -1: not
-  auto kern = p.causal ? flash_tc_kernel<E, true> : flash_tc_kernel<E, false>;
-  if (regs_ok[p.causal] == 0) {
+  static unsigned char configured[3][64] = {};
+  static int regs_ok[3] = {0, 0, 0};  // 0: not checked, 1: as planned, -1: not
+  const int form = p.win ? 2 : (p.causal ? 1 : 0);
+  auto kern = p.win ? flash_tc_kernel<E, false, true>
+                    : (p.causal ? flash_tc_kernel<E, true, false> : flash_tc_kernel<E, false, false>);
+  if (regs_ok[form] == 0) {
     // the register split assumes exactly REGS_LAUNCH registers per thread at
     // launch (a larger split would wait forever in setmaxnreg)
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return CA_EUNSUPPORTED;
-    regs_ok[p.causal] = fa.numRegs == C::REGS_LAUNCH ? 1 : -1;
+    regs_ok[form] = fa.numRegs == C::REGS_LAUNCH ? 1 : -1;
   }
-  if (regs_ok[p.causal] < 0) return CA_EUNSUPPORTED;
-  cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), C::SMEM_BYTES, configured[p.causal]);
+  if (regs_ok[form] < 0) return CA_EUNSUPPORTED;
+  cudaError_t e = smem_limit_once(reinterpret_cast<const void*>(kern), C::SMEM_BYTES, configured[form]);
   if (e != cudaSuccess) {
     *err = std::string("cudaFuncSetAttribute(flash_tc): ") + cudaGetErrorString(e);
     return CA_ECUDA;

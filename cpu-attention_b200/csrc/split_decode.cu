@@ -1,0 +1,102 @@
+// The split decode kernel's instantiations and launch.
+#include "split_launch.cuh"
+
+#include "split_decode.cuh"
+
+namespace ca {
+namespace {
+
+template <int KIND, typename QT, int E>
+cudaError_t launch(SplitParams prm, int ctas, int device, cudaStream_t stream) {
+  const int smem = split_smem_fixed<KIND, E>() + 4 * (prm.B + 1);
+  auto kern = split_decode_kernel<KIND, QT, E>;
+  static unsigned char configured[64] = {};
+  if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+  if (!configured[device]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         split_smem_fixed<KIND, E>() + 4 * (kSplitMaxBatch + 1));
+    if (e != cudaSuccess) return e;
+    configured[device] = 1;  // (a race sets the same value twice)
+  }
+  kern<<<ctas, 32 * kSplitWarps, smem, stream>>>(prm);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // the join of items cut by a CTA boundary starts as the decode drains
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(32 * kSplitMergeWarps);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, split_merge_kernel<KIND, QT, E>, prm);
+}
+
+template <int KIND, typename QT>
+cudaError_t by_dim(const SplitParams& prm, int head_dim, int ctas, int device, cudaStream_t s) {
+  switch (head_dim) {
+    case 32: return launch<KIND, QT, 32>(prm, ctas, device, s);
+    case 64: return launch<KIND, QT, 64>(prm, ctas, device, s);
+    default: return launch<KIND, QT, 128>(prm, ctas, device, s);
+  }
+}
+
+size_t piece_bytes(int head_dim) { return (size_t)(head_dim / 4 + 4) * 32 * 4; }
+
+}  // namespace
+
+size_t split_workspace_bytes(int head_dim, int sms) {
+  return (size_t)sms * kSplitCtasPerSm * (2 * piece_bytes(head_dim) + 16);
+}
+
+cudaError_t split_launch(const SplitCall& c, int sms, int device, cudaStream_t stream) {
+  const int ctas = sms * kSplitCtasPerSm;
+  const size_t es = c.q_dtype == CA_DTYPE_BF16 ? 2 : 4;
+  // sequences per launch: their tile counts fit shared memory and 32 bits
+  const long long row_tiles = std::max(1LL, c.table_width * (c.page / kSplitTile));
+  const long long most = std::max(1LL, std::min<long long>(kSplitMaxBatch, 0x7fffffffLL / row_tiles));
+  for (long long b0 = 0; b0 < c.batch; b0 += most) {
+    SplitParams prm{};
+    prm.q = static_cast<const char*>(c.q) + b0 * c.q_stride * (long long)es;
+    prm.q_stride = c.q_stride;
+    prm.kc = c.kc;
+    prm.vc = c.vc;
+    prm.ks = c.ks;
+    prm.vs = c.vs;
+    prm.num_blocks = c.num_blocks;
+    prm.lens = c.lens + b0;
+    prm.extra = (int)c.n_new;
+    prm.page_table = c.page_table + b0 * c.table_width;
+    prm.pt_stride = c.table_width;
+    prm.out = static_cast<char*>(c.out) + b0 * c.heads * c.head_dim * (long long)es;
+    prm.lse = c.lse ? c.lse + b0 * c.heads : nullptr;
+    prm.B = (int)std::min(most, c.batch - b0);
+    prm.H = (int)c.heads;
+    prm.Hk = (int)c.kv_heads;
+    prm.G = (int)(c.heads / c.kv_heads);
+    prm.NRG = (prm.G + 7) / 8;
+    prm.IH = prm.Hk * prm.NRG;
+    prm.page = (int)c.page;
+    prm.left = c.left < 0 ? -1 : (int)std::min<long long>(c.left, 0x7fffffff);
+    prm.sinks = (int)std::min<long long>(c.sinks, 0x7fffff00);
+    prm.c = c.c;
+    prm.min_chunk = 2;
+    prm.partial = static_cast<float*>(c.workspace);
+    prm.meta = reinterpret_cast<int*>(static_cast<char*>(c.workspace) + (size_t)ctas * 2 * piece_bytes(c.head_dim));
+    prm.status = c.status;
+    cudaError_t e;
+    if (c.cache_dtype == CA_DTYPE_E4M3)
+      e = c.q_dtype == CA_DTYPE_BF16 ? by_dim<kSplitE4m3, __nv_bfloat16>(prm, c.head_dim, ctas, device, stream)
+                                     : by_dim<kSplitE4m3, float>(prm, c.head_dim, ctas, device, stream);
+    else if (c.cache_dtype == CA_DTYPE_BF16)
+      e = by_dim<kSplitBf16, __nv_bfloat16>(prm, c.head_dim, ctas, device, stream);
+    else
+      e = by_dim<kSplitF32, float>(prm, c.head_dim, ctas, device, stream);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace ca

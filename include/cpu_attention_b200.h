@@ -39,6 +39,7 @@ extern "C" {
 /* ---- codes ------------------------------------------------------------ */
 #define CA_DTYPE_F32 0
 #define CA_DTYPE_BF16 1
+#define CA_DTYPE_E4M3 2 /* cache codes only (ca_decode_split, ca_append_8bit) */
 
 #define CA_OK 0
 #define CA_EDTYPE -1        /* dtype not fp32/bf16, or operands disagree      */
@@ -224,6 +225,111 @@ CA_API int ca_flash_ex(const void* q, const void* k, const void* v, void* out,
              const int32_t* cu_seqlens_k, int64_t total_q, int64_t total_k,
              float softmax_scale, int causal, int dtype, int32_t* status,
              void* stream);
+
+/* ---- prefill behind a sliding window ---------------------------------------
+ * ca_flash_ex (the reference declines windows, `flash_attn_interface.py:87-96`)
+ * with window_left, window_right and sink_tokens: row i, at position p = i +
+ * seq_k - seq_q of its sequence, sees key j when
+ *   j <= p + window_right  and  (j >= p - window_left  or  j < sink_tokens),
+ * so the first sink_tokens keys stay visible behind the window. -1 leaves a
+ * side unlimited; causal sets window_right to 0. With both sides -1 it is
+ * ca_flash_ex (sink_tokens then changes nothing). Key tiles that no row of a
+ * query tile sees are not read. Values have to be finite where a tile is read:
+ * a hidden key's weight is an exact zero, but zero times NaN is NaN.
+ */
+CA_API int ca_flash_window(const void* q, const void* k, const void* v,
+             void* out, float* lse, int64_t batch, int64_t seq_q, int64_t seq_k,
+             int64_t heads, int64_t kv_heads, int64_t head_dim,
+             const int64_t q_strides[3], const int64_t k_strides[3],
+             const int64_t v_strides[3], const int32_t* cu_seqlens_q,
+             const int32_t* cu_seqlens_k, int64_t total_q, int64_t total_k,
+             float softmax_scale, int causal, int64_t window_left,
+             int64_t window_right, int64_t sink_tokens, int dtype,
+             int32_t* status, void* stream);
+
+/* ---- caches held in 8 bits: the append ---------------------------------------
+ * The cache: k_cache/v_cache uint8 e4m3 codes [num_blocks, heads, page,
+ * head_dim] (both sides token-major, K is not transposed), k_scale/v_scale
+ * float32 [num_blocks, heads]; a value is code * scale of its block and head.
+ * Writes the new tokens of sequence i at positions lens[i], lens[i] + 1, ...
+ * through page_table [batch, table_width]. key/value of `dtype` (fp32 or bf16),
+ * heads and dims contiguous: dense, token j of sequence i at element i *
+ * seq_stride + j * token_stride, n_new tokens each; or packed (cu_new, device
+ * int32 [batch + 1]): rows [cu_new[i], cu_new[i + 1]) of total_new rows
+ * token_stride apart, at most n_new per sequence.
+ * The scale of a (block, head) that receives tokens becomes 2^e, the smallest
+ * e >= -126 that makes the largest finite |value| at most 448 codes' units, or
+ * stays where it was larger; a token at position 0 of the block starts it
+ * afresh (what it held is void). Where the scale grows, the block's other
+ * codes are rounded to it. Infinities are stored as the largest code. A block
+ * that two sequences' new tokens fall into must not be shared (copy it first:
+ * ca_copy_blocks). lens[i] < 0 skips sequence i; positions past the table and
+ * bad table entries are skipped and flagged (CA_STATUS_LENS / _TABLE).
+ */
+CA_API int ca_append_8bit(const void* key, const void* value, int64_t seq_stride,
+             int64_t token_stride, int64_t n_new, const int32_t* cu_new,
+             int64_t total_new, void* k_cache, void* v_cache, float* k_scale,
+             float* v_scale, int64_t num_blocks, const int32_t* lens,
+             const int32_t* page_table, int64_t table_width, int64_t batch,
+             int64_t heads, int64_t head_dim, int64_t page, int dtype,
+             int32_t* status, void* stream);
+
+/* ---- decode over 8-bit caches and behind a window ----------------------------
+ * One query token per sequence at the last attended position L - 1, as
+ * ca_decode_ex, over caches of cache_dtype: CA_DTYPE_E4M3 (ca_append_8bit's
+ * layout, k_scale/v_scale given, q fp32 or bf16) or q's own dtype (ca_store's
+ * layout, no scales). window_left >= 0: the row sees tokens t >= L - 1 -
+ * window_left and t < sink_tokens; pages wholly between them are not looked up,
+ * their table entries may be anything. window_left -1: all L tokens.
+ * n_new > 0: the new tokens k_new/v_new (q's dtype, kv_token_stride elements
+ * apart) are appended at lens[i] first and L = lens[i] + n_new.
+ * workspace: ca_decode_split_workspace_bytes() bytes, 16-byte aligned; its
+ * content needs no preparation and is not kept between calls, but calls that
+ * overlap in time must not share one. status: NULL or a device int32.
+ */
+CA_API size_t ca_decode_split_workspace_bytes(int64_t head_dim, int device);
+
+CA_API int ca_decode_split(const void* q, int64_t q_stride, void* k_cache,
+             void* v_cache, float* k_scale, float* v_scale, int64_t num_blocks,
+             const void* k_new, const void* v_new, int64_t kv_stride,
+             int64_t kv_token_stride, int64_t n_new, const int32_t* lens,
+             const int32_t* page_table, int64_t table_width, void* out,
+             float* lse, int64_t batch, int64_t heads, int64_t kv_heads,
+             int64_t head_dim, int64_t page, int q_dtype, int cache_dtype,
+             int64_t window_left, int64_t sink_tokens, float softmax_scale,
+             void* workspace, size_t workspace_bytes, int32_t* status,
+             void* stream);
+
+/* ---- moving blocks -------------------------------------------------------------
+ * ca_copy_blocks: for every pair (src, dst) of `pairs` (device int64 [n][2])
+ * and every one of `tensors` tensors [num_blocks, ...] whose blocks are
+ * block_bytes[t] contiguous bytes at base[t] (host arrays): block dst becomes
+ * block src. A negative id skips the pair; ids past the end are skipped and
+ * flagged (CA_STATUS_SLOT). No dst may be another pair's src or dst (which of
+ * the blocks' contents such a dst gets is not defined; nothing else is touched).
+ *
+ * ca_compact_blocks: packs the blocks in use. In use are the blocks of the
+ * table entries whose page starts below lens[i] and, with window_left >= 0, is
+ * not wholly between the first sink_tokens tokens and the window of a query at
+ * lens[i] - 1. With n of them, the k-th smallest id >= n in use moves to the
+ * k-th smallest free id < n, in every tensor. new_table gets the renumbered
+ * table, -1 in entries not in use (bad entries in use, flagged
+ * CA_STATUS_TABLE, too); used[0] = n. page_table is left as it was. workspace:
+ * ca_compact_workspace_bytes(num_blocks) bytes, no preparation needed.
+ * num_blocks up to 2^20.
+ */
+CA_API int ca_copy_blocks(void* const* base, const int64_t* block_bytes,
+             int64_t tensors, int64_t num_blocks, const int64_t* pairs,
+             int64_t n, int32_t* status, void* stream);
+
+CA_API size_t ca_compact_workspace_bytes(int64_t num_blocks);
+
+CA_API int ca_compact_blocks(void* const* base, const int64_t* block_bytes,
+             int64_t tensors, int64_t num_blocks, const int32_t* page_table,
+             const int32_t* lens, int64_t batch, int64_t table_width,
+             int64_t page, int64_t window_left, int64_t sink_tokens,
+             int32_t* new_table, int32_t* used, void* workspace,
+             size_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- runtime ------------------------------------------------------------ */
 /* The status word of a decode workspace (ORed CA_STATUS_* bits since the last

@@ -1,0 +1,615 @@
+"""Caches held in 8 bits, windows with first tokens and block moves on the B200,
+against float64 implementations (tests/serving.py) with derived bounds."""
+
+import math
+
+import pytest
+import torch
+
+import serving as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def api():
+    import cpu_attention
+    return cpu_attention
+
+
+def kernel():
+    from cpu_attention import _kernel
+    return _kernel
+
+
+def status(reset=True):
+    K = kernel()
+    return K.status(torch.device("cuda", torch.cuda.current_device()), reset=reset)
+
+
+def bytes_of(t):
+    """The bytes of a tensor [blocks, ...], one row per block."""
+    return t.contiguous().reshape(t.shape[0], -1).view(torch.uint8).cpu()
+
+
+# ------------------------------------------------------------------- append --
+def empty_8bit(blocks, heads, page, d, fill=0x7f):
+    c = torch.full((blocks, heads, page, d), fill, dtype=torch.uint8, device=DEV).view(S.F8)
+    return c, c.clone(), torch.zeros(blocks, heads, device=DEV), torch.zeros(blocks, heads, device=DEV)
+
+
+def check_append(kc, vc, ks, vs, want):
+    for got, ref in ((kc, want[0]), (vc, want[1])):
+        g = got.cpu().double()
+        assert torch.equal(torch.isnan(g), torch.isnan(ref))
+        assert torch.equal(g[~torch.isnan(g)], ref[~torch.isnan(ref)])
+    assert torch.equal(ks.cpu().double(), want[2]) and torch.equal(vs.cpu().double(), want[3])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 32), (32, 48), (128, 128)])
+def test_append_matches_definition(dtype, d, page):
+    """Appends of several sizes to the same caches, magnitudes growing and shrinking: codes and scales equal the
+    definition exactly (powers of two, one rounding)."""
+    g = torch.Generator().manual_seed(d + page)
+    heads, batch = 3, 4
+    width = 5
+    table = torch.randperm(batch * width + 2, generator=g)[:batch * width].reshape(batch, width).to(torch.int32)
+    blocks = batch * width + 2
+    kc, vc, ks, vs = empty_8bit(blocks, heads, page, d, 0)
+    want = [torch.zeros(blocks, heads, page, d, dtype=torch.float64) for _ in range(2)] \
+        + [torch.zeros(blocks, heads, dtype=torch.float64) for _ in range(2)]
+    lens = [0, page - 1, 3, page]
+    for n, size in ((1, 1.0), (1, 300.0), (page + 3, 1e-3), (2, 1e4), (1, 1e-30), (page // 2, 7.0)):
+        k, v = (torch.randn(batch, n, heads, d, generator=g).mul(size).to(dtype) for _ in range(2))
+        api().append_quantized(k.to(DEV), v.to(DEV), kc, vc, ks, vs, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                               table.to(DEV))
+        for x, r in enumerate((k, v)):
+            S.append(want[x], want[2 + x], [t.double() for t in r], lens, table.tolist(), page)
+        check_append(kc, vc, ks, vs, want)
+        lens = [a + n for a in lens]
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_append_packed_strided_and_left_out(dtype):
+    """Packed tokens as views of a fused projection (also at an odd element: no 16-byte loads), a sequence of zero
+    tokens, one left out by a negative length; blocks of nobody and slots behind a block's tokens stay as they were."""
+    g = torch.Generator().manual_seed(1)
+    heads, d, page = 2, 64, 16
+    news, lens = [5, 0, 40, 1, 9], [3, 7, 0, 31, -1]
+    total = sum(news)
+    for odd in (0, 1):
+        flat = torch.randn(total * (2 * heads * d + 8) + odd, generator=g).to(dtype).to(DEV)
+        fused = flat[odd:].view(total, 2 * heads * d + 8)
+        k, v = (fused[:, x * heads * d:(x + 1) * heads * d].view(total, heads, d) for x in range(2))
+        cu = torch.tensor([sum(news[:i]) for i in range(6)], dtype=torch.int32, device=DEV)
+        table = torch.randperm(24, generator=g)[:20].reshape(5, 4).to(torch.int32)
+        kc, vc, ks, vs = empty_8bit(24, heads, page, d, 0x31)
+        ks += 0.5
+        vs += 0.25
+        want = [kc.cpu().double(), vc.cpu().double(), ks.cpu().double(), vs.cpu().double()]
+        api().append_quantized(k, v, kc, vc, ks, vs, torch.tensor(lens, dtype=torch.int32, device=DEV), table.to(DEV),
+                               cu_seqlens_new=cu, max_seqlen_new=40)
+        for x, r in enumerate((k, v)):
+            rows = [r[sum(news[:i]):sum(news[:i + 1])].cpu().double() for i in range(5)]
+            S.append(want[x], want[2 + x], rows, lens, table.tolist(), page)
+        check_append(kc, vc, ks, vs, want)
+    # offsets and lengths on the host
+    api().append_quantized(k, v, kc, vc, ks, vs, torch.tensor(lens, dtype=torch.int32), table, cu_seqlens_new=cu.cpu())
+    for x, r in enumerate((k, v)):
+        rows = [r[sum(news[:i]):sum(news[:i + 1])].cpu().double() for i in range(5)]
+        S.append(want[x], want[2 + x], rows, lens, table.tolist(), page)
+    check_append(kc, vc, ks, vs, want)
+    assert status() == 0
+
+
+def test_append_infinities_nan_and_zeros():
+    """An infinity becomes the largest code and sets no scale, NaN stays NaN, zeros alone take the smallest scale."""
+    kc, vc, ks, vs = empty_8bit(2, 1, 16, 32, 0)
+    k = torch.zeros(1, 2, 1, 32)
+    k[0, 0, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, 3.0])
+    v = torch.zeros(1, 2, 1, 32)
+    api().append_quantized(k.to(DEV), v.to(DEV), kc, vc, ks, vs, torch.zeros(1, dtype=torch.int32, device=DEV),
+                           torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    s = S.fit_scale(torch.tensor([3.0]))
+    assert ks[0, 0].item() == s and vs[0, 0].item() == 2.0 ** -126
+    row = kc[0, 0, 0].cpu().double()
+    assert row[0] == 448 and row[1] == -448 and torch.isnan(row[2]) and row[3] * s == 3.0
+    assert (vc[0, 0, :2].cpu().double() == 0).all()
+
+
+def test_append_out_of_place_is_flagged():
+    """Positions past the table and bad entries are skipped and flagged, the rest is written."""
+    K = kernel()
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(3, 20, 1, 32, generator=g).to(DEV) for _ in range(2))
+    kc, vc, ks, vs = empty_8bit(8, 1, 16, 32, 0)
+    table = torch.tensor([[0, 1], [2, 99], [-5, 3]], dtype=torch.int32, device=DEV)
+    status()
+    api().append_quantized(k, v, kc, vc, ks, vs, torch.tensor([16, 0, 0], dtype=torch.int32, device=DEV), table)
+    assert status() == K.STATUS_LENS | K.STATUS_TABLE
+    want = [torch.zeros(8, 1, 16, 32, dtype=torch.float64) for _ in range(2)] \
+        + [torch.zeros(8, 1, dtype=torch.float64) for _ in range(2)]
+    for x, r in enumerate((k, v)):
+        S.append(want[x], want[2 + x], [t.cpu().double() for t in r], [16, 0, 0], table.tolist(), 16)
+    check_append(kc, vc, ks, vs, want)
+    # more tokens in a packed sequence than stated: the first ones are stored
+    cu = torch.tensor([0, 20], dtype=torch.int32, device=DEV)
+    api().append_quantized(k[0], v[0], kc, vc, ks, vs, torch.zeros(1, dtype=torch.int32, device=DEV), table[:1], cu, 4)
+    assert status() == K.STATUS_LENS
+
+
+# ------------------------------------------------------------------- decode --
+LENS = [0, 1, 15, 16, 17, 100, 333, 0, 1030]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("h,hk", [(4, 4), (6, 2), (8, 1), (20, 2)])
+def test_decode_8bit(dtype, d, page, h, hk):
+    pc = S.Paged("8bit", LENS, hk, d, page, dtype, seed=d + page + h)
+    q = torch.randn(len(LENS), 1, h, d, generator=torch.Generator().manual_seed(h)).to(dtype).to(DEV)
+    out, lse = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt,
+                                             return_softmax_lse=True, **pc.opts())
+    assert out.shape == q.shape and out.dtype == dtype
+    S.check_decode(out, lse, q, pc, h)
+    assert status() == 0
+    again = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt, **pc.opts())
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("kind", ["8bit", "bf16", "fp32"])
+@pytest.mark.parametrize("d,page,h,hk", [(128, 16, 8, 2), (64, 32, 4, 4), (32, 48, 18, 2)])
+@pytest.mark.parametrize("left,sinks", [(0, 0), (0, 1), (15, 4), (16, 16), (100, 17), (5000, 3), (64, 0), (-1, 7),
+                                        (31, 400)])
+def test_decode_window(kind, d, page, h, hk, left, sinks):
+    dtype = FP32 if kind == "fp32" else BF16
+    pc = S.Paged(kind, LENS, hk, d, page, dtype, seed=left + sinks, left=left, sinks=sinks)
+    q = torch.randn(len(LENS), 1, h, d, generator=torch.Generator().manual_seed(h)).to(dtype).to(DEV)
+    out, lse = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt,
+                                             window_size=(left, 0), sink_tokens=sinks, return_softmax_lse=True,
+                                             **pc.opts())
+    S.check_decode(out, lse, q, pc, h)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("kind", ["8bit", "bf16", "fp32"])
+@pytest.mark.parametrize("lens,h,hk", [([40000], 8, 1), ([9000, 1, 0, 12345], 32, 8), ([700] * 40, 4, 4)])
+def test_decode_long_and_split(kind, lens, h, hk):
+    """Items that many warps and CTAs share: joined in order, the same bits each time."""
+    dtype = FP32 if kind == "fp32" else BF16
+    pc = S.Paged(kind, lens, hk, 128, 16, dtype, seed=3, left=-1)
+    q = torch.randn(len(lens), 1, h, 128, generator=torch.Generator().manual_seed(5)).to(dtype).to(DEV)
+    call = lambda: api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L,  # noqa: E731
+                                                 page_table=pc.bt, sink_tokens=0, return_softmax_lse=True, **pc.opts())
+    out, lse = call()
+    S.check_decode(out, lse, q, pc, h)
+    for _ in range(3):
+        o2, l2 = call()
+        assert torch.equal(out, o2) and torch.equal(lse, l2)
+
+
+def test_decode_large_scores_scales_and_queries():
+    """Scores far apart, queries of 2^-120 to 2^100, scales from 2^-100 to 2^20, a negative softmax scale, an explicit
+    one, a block of scale 0."""
+    lens, h = [200, 37, 64], 4
+    for dtype in (BF16, FP32):
+        pc = S.Paged("8bit", lens, 2, 64, 16, dtype, seed=4)
+        for x in range(2):
+            e = torch.randint(-100 if x else -30, 21 if x else 3, pc.scale[x].shape,
+                              generator=torch.Generator().manual_seed(x))
+            pc.scale[x] = torch.exp2(e.double())
+            pc.scale[x][pc.table[0][1]] = 0.0
+        pc.k_scale, pc.v_scale = (s.float().to(DEV) for s in pc.scale)
+        base = torch.randn(3, 1, h, 64, generator=torch.Generator().manual_seed(9))
+        for size, scale in ((1.0, None), (2.0 ** -120, None), (2.0 ** 100, 2.0 ** -100), (1.0, -0.05), (1.0, 0.0)):
+            q = (base * size).to(dtype).to(DEV)
+            out, lse = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt,
+                                                     softmax_scale=scale, return_softmax_lse=True, **pc.opts())
+            S.check_decode(out, lse, q, pc, h, scale)
+
+
+@pytest.mark.parametrize("kind", ["8bit", "bf16", "fp32"])
+@pytest.mark.parametrize("n", [1, 3, 21])
+@pytest.mark.parametrize("window", [None, (20, 4)])
+def test_decode_appends(kind, n, window):
+    """k/v in the call: the caches afterwards equal the two-step route's, and the row sees its new tokens."""
+    dtype = FP32 if kind == "fp32" else BF16
+    lens, h, hk, d, page = [0, 15, 16, 100, 31], 4, 2, 64, 16
+    left, sinks = window if window else (-1, 0)
+    pc = S.Paged(kind, lens, hk, d, page, dtype, seed=n * 2, left=left, sinks=sinks, room=n)
+    if kind == "8bit":  # what was never written must be a number: the append keeps what a block holds
+        for c in (pc.k_cache, pc.v_cache):
+            u = c.view(torch.uint8)
+            u[(u & 0x7f) == 0x7f] = 0
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(len(lens), n, hk, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    q = torch.randn(len(lens), 1, h, d, generator=g).to(dtype).to(DEV)
+    opts = dict(window_size=(left, 0), sink_tokens=sinks) if window else (dict() if kind == "8bit"
+                                                                         else dict(sink_tokens=0))
+    k2, v2 = pc.k_cache.clone(), pc.v_cache.clone()
+    s2 = [None if s is None else s.clone() for s in (pc.k_scale, pc.v_scale)]
+    # the call's own route first on the live caches
+    out = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, k=k, v=v, cache_seqlens=pc.L, page_table=pc.bt,
+                                        **pc.opts(), **opts)
+    if kind == "8bit":
+        api().append_quantized(k, v, k2, v2, *s2, pc.L, pc.bt)
+        assert torch.equal(s2[0], pc.k_scale) and torch.equal(s2[1], pc.v_scale)
+        pc.scale = [s.cpu().double() for s in (pc.k_scale, pc.v_scale)]
+    else:
+        pos = pc.L.long()[:, None] + torch.arange(n, device=DEV)
+        slots = pc.bt.long().gather(1, pos // page) * page + pos % page
+        api().reshape_and_cache(k.flatten(0, 1), v.flatten(0, 1), k2, v2, slots.flatten())
+    assert torch.equal(bytes_of(k2), bytes_of(pc.k_cache)) and torch.equal(bytes_of(v2), bytes_of(pc.v_cache))
+    pc.rows = [S.unpack(c.cpu().double() if kind == "8bit" else c.cpu(), x == 0, kind).double()
+               for x, c in enumerate((pc.k_cache, pc.v_cache))]
+    S.check_decode(out, None, q, pc, h, lens=[a + n for a in lens])
+    assert status() == 0
+
+
+def test_decode_negative_length_and_bad_table():
+    """A negative length and bad entries read nothing out of place: zeros, or the rest of the row, and a flag."""
+    K = kernel()
+    pc = S.Paged("8bit", [40, 40, 40], 2, 64, 16, BF16, seed=6)
+    q = torch.randn(3, 1, 2, 64, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
+    bt = pc.bt.clone()
+    bt[1, 1] = -3
+    bt[2, 0] = 1 << 30
+    status()
+    out = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=bt, **pc.opts())
+    assert status() == K.STATUS_TABLE
+    good = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt, **pc.opts())
+    assert torch.equal(out[0], good[0]) and torch.isfinite(out).all()
+    L = torch.tensor([40, -1, 400], dtype=torch.int32, device=DEV)
+    out = api().flash_attn_with_kvcache(q[:2], pc.k_cache, pc.v_cache, cache_seqlens=L[:2], page_table=pc.bt[:2],
+                                        **pc.opts())
+    assert torch.equal(out[0], good[0]) and (out[1] == 0).all() and status() == 0
+    api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=L, page_table=pc.bt, **pc.opts())
+    assert status() & K.STATUS_LENS
+
+
+def test_decode_large_batch():
+    """More sequences than one launch takes."""
+    B = 9000
+    g = torch.Generator().manual_seed(0)
+    codes = torch.randn(64, 1, 16, 32, generator=g)
+    kc, vc = codes.to(S.F8).to(DEV), codes.flip(0).contiguous().to(S.F8).to(DEV)
+    one = torch.ones(64, 1, device=DEV)
+    bt = torch.randint(0, 64, (B, 2), generator=g).to(torch.int32)
+    L = torch.randint(0, 33, (B,), generator=g).to(torch.int32)
+    q = torch.randn(B, 1, 1, 32, generator=g).bfloat16()
+    out = api().flash_attn_with_kvcache(q.to(DEV), kc, vc, cache_seqlens=L.to(DEV), page_table=bt.to(DEV),
+                                        k_descale=one, v_descale=one)
+    for i in list(range(0, B, 611)) + [8191, 8192, 8999]:
+        one_row = api().flash_attn_with_kvcache(q[i:i + 1].to(DEV), kc, vc, cache_seqlens=L[i:i + 1].to(DEV),
+                                                page_table=bt[i:i + 1].to(DEV), k_descale=one, v_descale=one)
+        assert (out[i] - one_row[0]).abs().max() <= 2 ** -7 * one_row.abs().max() + 1e-6, i
+        if L[i] == 0:
+            assert (out[i] == 0).all()
+
+
+def test_decode_strided_queries_and_host_indices():
+    """q as a view of a fused projection, lengths and table on the host, an int length, cache_batch_idx."""
+    pc = S.Paged("8bit", [50, 50], 2, 64, 16, BF16, seed=8)
+    fused = torch.randn(2, 1, 3, 4, 64, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
+    q = fused[:, :, 1]
+    ref = api().flash_attn_with_kvcache(q.contiguous(), pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt,
+                                        **pc.opts())
+    for L, bt in ((pc.L, pc.bt), (pc.L.cpu(), pc.bt.cpu()), (50, pc.bt)):
+        out = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=L, page_table=bt, **pc.opts())
+        assert torch.equal(out, ref)
+    out = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, block_table=pc.bt.flip(0),
+                                        cache_batch_idx=torch.tensor([1, 0], device=DEV), **pc.opts())
+    assert torch.equal(out, ref)
+    # the ctypes path answers the same
+    from cpu_attention import _kernel as K, _native
+    fast, K._FAST = K.fastpath(), False
+    try:
+        got = _native.decode_split(0, q, pc.k_cache, pc.v_cache, None, None, pc.k_scale, pc.v_scale, pc.L, pc.bt, -1, 0,
+                                   None)
+    finally:
+        K._FAST = fast
+    assert torch.equal(got, ref)
+
+
+def test_decode_graphs_and_streams():
+    """Two captured steps (append and attend) replayed side by side on two streams, with fresh inputs: equal to eager
+    calls; nothing is shared between them."""
+    C = api()
+    steps = []
+    for x in range(2):
+        pc = S.Paged("8bit", [700, 50, 1200, 16], 4, 128, 16, BF16, seed=10 + 2 * x, room=1)
+        for c in (pc.k_cache, pc.v_cache):
+            u = c.view(torch.uint8)
+            u[(u & 0x7f) == 0x7f] = 0
+        g = torch.Generator().manual_seed(x)
+        q = torch.randn(4, 1, 16, 128, generator=g).bfloat16().to(DEV)
+        k, v = (torch.randn(4, 1, 4, 128, generator=g).bfloat16().to(DEV) for _ in range(2))
+        call = lambda pc=pc, q=q, k=k, v=v: C.flash_attn_with_kvcache(  # noqa: E731
+            q, pc.k_cache, pc.v_cache, k=k, v=v, cache_seqlens=pc.L, page_table=pc.bt, **pc.opts())
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = call()
+        steps.append((pc, q, k, v, call, s, graph, out))
+    for r in range(3):
+        g = torch.Generator().manual_seed(100 + r)
+        for pc, q, k, v, call, s, graph, out in steps:
+            for t in (q, k, v):
+                t.copy_(torch.randn(t.shape, generator=g).bfloat16())
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for pc, q, k, v, call, s, graph, out in steps:
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for pc, q, k, v, call, s, graph, out in steps:
+            assert torch.equal(out, call())
+
+
+# ------------------------------------------------------------------ prefill --
+def check_prefill(out, lse, q, k, v, left, right, sinks, causal, scale=None):
+    """One sequence: out [lq, h, d] against the definition. Weights enter the bf16 kernel's second product rounded to
+    bf16 (2^-8), the fp32 kernel's not at all; up to 2^8 times the largest is the bf16 kernel's slack, which
+    changes no relative error."""
+    lq, h, d = q.shape
+    lk, kv = k.shape[:2]
+    scale = d ** -0.5 if scale is None else scale
+    i, j = torch.arange(lq)[:, None] + lk - lq, torch.arange(lk)[None]
+    r = 0 if causal else right
+    seen = torch.ones(lq, lk, dtype=torch.bool)
+    if left >= 0:
+        seen &= (j >= i - left) | (j < sinks)
+    if r >= 0:
+        seen &= j <= i + r
+    weight = 2.0 ** -8 if q.dtype == BF16 else 0.0
+    for x in range(h):
+        ref, z, spread, top = S.attention(q[:, x].double().cpu(), k[:, x * kv // h].double().cpu(),
+                                          v[:, x * kv // h].double().cpu(), seen, scale)
+        tol = S.bound(ref, spread, top, d, lk * 16, q.dtype, weight)
+        err = (out[:, x].double().cpu() - ref).abs()
+        assert (err <= tol).all(), (x, err.max().item(), (err / tol).max().item())
+        if lse is not None:
+            zz = lse[x].double().cpu()
+            none = ~seen.any(-1)
+            assert torch.equal(torch.isneginf(zz), none)
+            assert ((zz - z)[~none].abs() <= 1e-4).all()
+
+
+WINDOWS = [(0, 0, 0), (5, 0, 1), (64, 0, 4), (100, 30, 0), (127, -1, 130), (-1, 10, 3), (300, 0, 17), (40, 0, 1000),
+           (0, 300, 5)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("left,right,sinks", WINDOWS)
+@pytest.mark.parametrize("lq,lk,h,hk,d", [(1, 1, 1, 1, 64), (300, 300, 2, 1, 128), (77, 640, 2, 2, 64),
+                                          (700, 513, 2, 2, 32), (1100, 1100, 1, 1, 64)])
+def test_prefill_window(dtype, left, right, sinks, lq, lk, h, hk, d):
+    g = torch.Generator().manual_seed(lq + left)
+    q = torch.randn(2, lq, h, d, generator=g).to(dtype).to(DEV)
+    k, v = (torch.randn(2, lk, hk, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    for causal in (False, True):
+        out, lse = api().flash_attn_func(q, k, v, causal=causal, window_size=(left, right), sink_tokens=sinks,
+                                         return_attn_probs=True)
+        for b in range(2):
+            check_prefill(out[b], lse[b], q[b], k[b], v[b], left, right, sinks, causal)
+        assert torch.equal(out, api().flash_attn_func(q, k, v, causal=causal, window_size=(left, right),
+                                                      sink_tokens=sinks))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("left,right,sinks", [(16, 0, 4), (200, 0, 0), (60, 60, 140)])
+def test_prefill_window_packed(dtype, left, right, sinks):
+    """Packed sequences, one empty: each equals a dense call on it alone, bit for bit; a layout TMA cannot read too."""
+    C = api()
+    lens = [1, 300, 0, 77, 520]
+    g = torch.Generator().manual_seed(left)
+    t, h, hk, d = sum(lens), 4, 2, 64
+    cu = torch.tensor([sum(lens[:i]) for i in range(6)], dtype=torch.int32, device=DEV)
+    wide = torch.randn(t, h + 2 * hk, d + 4, generator=g).to(dtype).to(DEV)
+    for q, k, v in ((wide[:, :h, :d].contiguous(), wide[:, h:h + hk, :d].contiguous(), wide[:, h + hk:, :d].contiguous()),
+                    (wide[:, :h, 1:d + 1], wide[:, h:h + hk, 1:d + 1], wide[:, h + hk:, 1:d + 1])):
+        for causal in (True, False):
+            opts = dict(causal=causal, window_size=(left, right), sink_tokens=sinks, return_attn_probs=True)
+            out, lse = C.flash_attn_varlen_func(q, k, v, cu, cu, 520, 520, **opts)
+            for i, n in enumerate(lens):
+                if n == 0:
+                    continue
+                a, z = int(cu[i]), int(cu[i + 1])
+                check_prefill(out[a:z], lse[:, a:z], q[a:z], k[a:z], v[a:z], left, right, sinks, causal)
+                dense, dl = C.flash_attn_func(q[a:z][None], k[a:z][None], v[a:z][None], **opts)
+                assert torch.equal(out[a:z], dense[0]) and torch.equal(lse[:, a:z], dl[0])
+
+
+def test_prefill_window_that_hides_nothing():
+    """A window as long as the sequences gives the result of no window (fp32: the same tiles, the same bits)."""
+    g = torch.Generator().manual_seed(0)
+    for dtype in (BF16, FP32):
+        q, k, v = (torch.randn(1, 400, 2, 64, generator=g).to(dtype).to(DEV) for _ in range(3))
+        plain = api().flash_attn_func(q, k, v, causal=True)
+        wide = api().flash_attn_func(q, k, v, causal=True, window_size=(10 ** 12, 0), sink_tokens=3)
+        assert torch.equal(plain, wide)
+        assert torch.equal(plain, api().flash_attn_func(q, k, v, causal=True, sink_tokens=7))
+
+
+# -------------------------------------------------------------- block moves --
+def layer_caches(blocks, layers, g, page=16):
+    out = []
+    for _ in range(layers):
+        out += [torch.randn(blocks, 2, page, 32, generator=g).bfloat16().to(DEV),
+                torch.randn(blocks, 2, page, 64, generator=g).to(S.F8).to(DEV),
+                torch.randn(blocks, 3, generator=g).to(DEV), torch.randint(0, 9, (blocks,), generator=g).to(DEV),
+                torch.randint(0, 255, (blocks, 7), generator=g).to(torch.uint8).to(DEV)]
+    return out
+
+
+@pytest.mark.parametrize("layers", [1, 30])
+def test_copy_blocks(layers):
+    g = torch.Generator().manual_seed(layers)
+    caches = layer_caches(40, layers, g)
+    before = [bytes_of(c) for c in caches]
+    pairs = torch.tensor([[3, 9], [3, 10], [-1, 4], [5, -7], [0, 39], [8, 8 + 12]], dtype=torch.int64)
+    for where in (DEV, "cpu"):
+        api().copy_blocks(caches, pairs.to(where))
+        for c, was in zip(caches, before):
+            now, want = bytes_of(c), was.clone()
+            for a, b in pairs.tolist():
+                if a >= 0 and b >= 0:
+                    want[b] = was[a]
+            assert torch.equal(now, want)
+    status()
+    api().copy_blocks(caches, torch.tensor([[1, 40], [1 << 40, 2], [6, 7]], device=DEV))
+    assert status() == kernel().STATUS_SLOT
+    assert torch.equal(bytes_of(caches[0])[7], before[0][6]) and torch.equal(bytes_of(caches[0])[2], before[0][2])
+    api().copy_blocks(caches, torch.zeros(0, 2, dtype=torch.int64, device=DEV))
+    api().copy_blocks([], torch.zeros(0, 2, dtype=torch.int64, device=DEV))
+    api().copy_blocks(caches[0], torch.tensor([[0, 1]], device=DEV))
+    assert torch.equal(bytes_of(caches[0])[1], before[0][0])
+
+
+def plain_compact(table, lens, page, blocks, left, sinks):
+    live = [[p * page < n and (left < 0 or (p + 1) * page > n - 1 - left or p * page < sinks) for p in range(len(row))]
+            for row, n in zip(table, lens)]
+    used = {b for row, on in zip(table, live) for b, x in zip(row, on) if x and 0 <= b < blocks}
+    free = [b for b in range(len(used)) if b not in used]
+    moves = dict(zip(sorted(b for b in used if b >= len(used)), free))
+    new = [[moves.get(b, b) if x and 0 <= b < blocks else -1 for b, x in zip(row, on)]
+           for row, on in zip(table, live)]
+    return new, len(used), moves
+
+
+@pytest.mark.parametrize("blocks,batch,width,left,sinks", [(50, 6, 5, -1, 0), (1000, 7, 40, 100, 4), (33, 1, 1, -1, 0),
+                                                           (40000, 20, 1500, 300, 33), (64, 5, 9, 0, 0)])
+def test_compact_blocks(blocks, batch, width, left, sinks):
+    g = torch.Generator().manual_seed(blocks)
+    page = 16
+    caches = layer_caches(blocks, 1, g)
+    before = [bytes_of(c) for c in caches]
+    table = torch.randperm(blocks, generator=g)
+    table = table[torch.randint(0, blocks, (batch, width), generator=g)] if batch * width > blocks // 2 else \
+        table[:batch * width].reshape(batch, width)
+    lens = torch.randint(0, width * page + 1, (batch,), generator=g)
+    if batch > 2:
+        table[1, :3] = table[0, :3]  # shared
+    table, lens = table.to(torch.int32), lens.to(torch.int32)
+    new, used = api().compact_blocks(caches, table.to(DEV), lens.to(DEV), page, window_size=(left, 0), sink_tokens=sinks)
+    want, n, moves = plain_compact(table.tolist(), lens.tolist(), page, blocks, left, sinks)
+    assert used.tolist() == [n] and new.tolist() == want
+    for c, was in zip(caches, before):
+        ref = was.clone()
+        for a, b in moves.items():
+            ref[b] = was[a]
+        assert torch.equal(bytes_of(c), ref)
+    # packed already: nothing moves
+    again, used = api().compact_blocks(caches, new, lens.to(DEV), page, window_size=(left, 0), sink_tokens=sinks)
+    assert torch.equal(again, new) and used.tolist() == [n]
+
+
+def test_compact_flags_bad_entries():
+    K = kernel()
+    g = torch.Generator().manual_seed(0)
+    caches = layer_caches(10, 1, g)
+    table = torch.tensor([[9, 99], [-2, 8]], dtype=torch.int32, device=DEV)
+    status()
+    new, used = api().compact_blocks(caches, table, torch.tensor([20, 32], dtype=torch.int32, device=DEV), 16)
+    assert status() == K.STATUS_TABLE
+    assert new.tolist() == [[1, -1], [-1, 0]] and used.tolist() == [2]
+    api().compact_blocks(caches, table[:1], torch.tensor([100], dtype=torch.int32, device=DEV), 16)
+    assert status() & K.STATUS_LENS
+    empty, used = api().compact_blocks(caches, table[:0], torch.zeros(0, dtype=torch.int32, device=DEV), 16)
+    assert empty.shape == (0, 2) and used.tolist() == [0]
+
+
+# ----------------------------------------------------------- a run together --
+@pytest.mark.parametrize("kind", ["8bit", "bf16"])
+def test_serving_run(kind):
+    """Prompts enter the cache, sequences decode behind a window, one forks, the pool is packed, decoding goes on: the
+    outputs are those of the same tokens attended in float64, whatever moved."""
+    C = api()
+    g = torch.Generator().manual_seed(5)
+    h, hk, d, page, left, sinks = 8, 2, 64, 16, 40, 4
+    lens = [70, 5, 33]
+    width, blocks = 16, 80
+    table = torch.full((4, width), -1, dtype=torch.int32)
+    free = torch.randperm(blocks, generator=g).tolist()
+    if kind == "8bit":
+        kc, vc, ks, vs = empty_8bit(blocks, hk, page, d, 0)
+        caches = [kc, vc, ks, vs]
+        opts = dict(k_descale=ks, v_descale=vs)
+    else:
+        kc, vc = (torch.zeros(blocks, hk, page, d, dtype=BF16, device=DEV) for _ in range(2))
+        caches, opts = [kc, vc], {}
+
+    def grow(i, n):
+        for p in range(-(-n // page)):
+            if table[i, p] < 0 and (p * page < sinks or (p + 1) * page > n - 1 - left):
+                table[i, p] = free.pop()
+
+    hist = [[torch.randn(n, hk, d, generator=g).bfloat16() for _ in range(2)] for n in lens]
+    for i, n in enumerate(lens):
+        for p in range(-(-n // page)):
+            table[i, p] = free.pop()
+    cu = torch.tensor([0, 70, 75, 108], dtype=torch.int32, device=DEV)
+    key, value = (torch.cat([x[s] for x in hist]).to(DEV) for s in range(2))
+    if kind == "8bit":
+        C.append_quantized(key, value, kc, vc, ks, vs, torch.zeros(3, dtype=torch.int32, device=DEV),
+                           table[:3].to(DEV), cu, 70)
+    else:
+        pos = torch.cat([torch.arange(n) for n in lens])
+        seq = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)])
+        C.reshape_and_cache(key, value, kc, vc, (table[seq, pos // page].long() * page + pos % page).to(DEV))
+    lens = lens + [0]
+    hist.append([torch.zeros(0, hk, d).bfloat16() for _ in range(2)])
+    # what 8 bits lose: a value is off by at most 2^-4 of itself, or half a step of the smallest code's unit; three
+    # scale growths at most (each rounds small codes again). Bounded here against the tokens themselves.
+    for step in range(50):
+        if step == 20:  # sequence 3 forks sequence 0: whole pages shared, the open one copied
+            open_page = lens[0] // page
+            table[3] = table[0]
+            if lens[0] % page:
+                fresh = free.pop()
+                C.copy_blocks(caches, torch.tensor([[int(table[0, open_page]), fresh]], device=DEV))
+                table[3, open_page] = fresh
+            lens[3], hist[3] = lens[0], [x.clone() for x in hist[0]]
+        if step == 35:  # free what the window has left, pack the rest
+            L = torch.tensor(lens, dtype=torch.int32, device=DEV)
+            new, used = C.compact_blocks(caches, table.to(DEV), L, page, window_size=(left, 0), sink_tokens=sinks)
+            table = new.cpu()
+            free = list(range(int(used), blocks))
+            assert int(used) < 30
+        rows = [0, 1, 2] if step < 20 else [0, 1, 2, 3]
+        for i in rows:
+            grow(i, lens[i] + 1)
+        q = torch.randn(len(rows), 1, h, d, generator=g).bfloat16()
+        k, v = (torch.randn(len(rows), 1, hk, d, generator=g).bfloat16() for _ in range(2))
+        out = C.flash_attn_with_kvcache(q.to(DEV), kc, vc, k=k.to(DEV), v=v.to(DEV),
+                                        cache_seqlens=torch.tensor([lens[i] for i in rows], dtype=torch.int32,
+                                                                   device=DEV),
+                                        page_table=table[rows].to(DEV), window_size=(left, 0), sink_tokens=sinks, **opts)
+        for x, i in enumerate(rows):
+            hist[i] = [torch.cat([hist[i][0], k[x]]), torch.cat([hist[i][1], v[x]])]
+            lens[i] += 1
+            if step % 7 and step not in (20, 35, 36):
+                continue
+            pos = torch.tensor(S.seen_decode(lens[i], left, sinks))
+            for a in range(hk):
+                kk, vv = (hist[i][s][pos, a].double() for s in range(2))
+                qq = q[x, 0, a * 4:(a + 1) * 4].double()
+                ref, _, spread, top = S.attention(qq, kk, vv, torch.ones(4, len(pos), dtype=torch.bool), d ** -0.5)
+                # scores move by at most (2^-4 + growth) of sum |q||k|; each weight by the exponential of twice that;
+                # values by 2^-4 of themselves plus two units of the smallest step of a block of N(0, 1) values
+                eight = kind == "8bit"
+                shift = top * 1.1 * 2 ** -4 if eight else torch.zeros_like(top)
+                tol = S.bound(ref, spread, top, d, len(pos), BF16, 2.0 ** -11 if eight else 2.0 ** -16)
+                tol = tol + (spread + 0.05) * (torch.expm1(2 * shift)[:, None] + (2 ** -4 if eight else 0)) + 1e-3
+                err = (out[x, 0, a * 4:(a + 1) * 4].double().cpu() - ref).abs()
+                assert (err <= tol).all(), (step, i, err.max().item())
+    assert status() == 0
