@@ -24,7 +24,7 @@ cudaError_t launch(SplitParams prm, int ctas, int device, cudaStream_t stream) {
   // the join of items cut by a CTA boundary starts as the decode drains
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(32 * kSplitMergeWarps);
+  cfg.blockDim = dim3(32 * kSplitMergeShares * (E / 16));
   cfg.stream = stream;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -83,8 +83,9 @@ cudaError_t split_launch(const SplitCall& c, int sms, int device, cudaStream_t s
     prm.sinks = (int)std::min<long long>(c.sinks, 0x7fffff00);
     prm.c = c.c;
     prm.min_chunk = 2;
+    prm.q_vec = (reinterpret_cast<uintptr_t>(prm.q) % 16 == 0) && (c.q_stride * es) % 16 == 0;
     prm.partial = static_cast<float*>(c.workspace);
-    prm.meta = reinterpret_cast<int*>(static_cast<char*>(c.workspace) + (size_t)ctas * 2 * piece_bytes(c.head_dim));
+    prm.meta = reinterpret_cast<int*>(prm.partial + (size_t)ctas * 2 * piece_bytes(c.head_dim) / 4);
     prm.status = c.status;
     cudaError_t e;
     if (c.cache_dtype == CA_DTYPE_E4M3)

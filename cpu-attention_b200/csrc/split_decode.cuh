@@ -34,12 +34,10 @@
 //                 byte by byte (8-bit) or half by half (bf16) so that a register
 //                 holds one dim of two keys; P^T is S^T through movmatrix.
 //   8-bit codes widen exactly to f16; q is scaled by a power of two per row so
-//   that f16 holds it. P is taken against the tile's own maximum, so a tile's
-//   largest weight is 1 whatever came before, and enters as one f16 value for
-//   bf16 outputs (2^-12 of the weight, against 2^-9 of the output's rounding)
-//   and as a value plus its rest for fp32 ones and for bf16 caches.
-//   The tile's product is scaled by s_v * 2^(m_tile - m) when it is added, so
-//   any scale a user stores is followed.
+//   that f16 holds it. P enters as one f16 value for bf16 outputs (2^-12 of the
+//   weight, against 2^-9 of the output's rounding) and as a value plus its rest
+//   for fp32 ones and for bf16 caches; s_v enters with it, against a unit that
+//   follows the scales a user stores (fp32 outputs: when the tile is added).
 // fp32 caches run the same tiles on FMAs.
 //
 // Loads of tile n+1 are issued as soon as the registers of tile n are free: 12
@@ -59,8 +57,15 @@ enum SplitKind { kSplitF32 = 0, kSplitBf16 = 1, kSplitE4m3 = 2 };
 constexpr int kSplitWarps = 6;        // warps per CTA
 constexpr int kSplitCtasPerSm = 2;    // CTAs per SM
 constexpr int kSplitTile = 16;        // tokens per tile
-constexpr int kSplitMaxBatch = 8192;  // sequences per launch (their tile counts sit in shared memory)
-constexpr int kSplitMergeWarps = 4;
+constexpr int kSplitMaxBatch = 1024;  // sequences per launch (their tile counts sit in shared memory)
+constexpr int kSplitRing = 16384;     // bytes of tiles a warp has in flight
+constexpr int kSplitMeta = 64;        // tiles whose places a warp keeps
+constexpr int kSplitAhead = 2;        // tiles ahead whose lines are brought to L2 (at most 16)
+// Weights are kept as 2^(x - m + kUp), m a reference that a column's largest x
+// may pass by kSlack before it moves (a vote per tile, no reduction): up to 2^14
+// for f16, whose smallest step is then 2^-30 of the reference's weight.
+constexpr float kUp = 6.f, kSlack = 8.f;
+constexpr int kSplitMergeShares = 4;
 
 struct SplitParams {
   const void* q;
@@ -81,8 +86,9 @@ struct SplitParams {
   int page;
   int left, sinks;  // left < 0: no window
   float c;          // softmax_scale * log2(e)
-  int min_chunk;    // tiles a warp takes at least
-  float* partial;   // [2 * CTAs] pieces of items cut by a CTA boundary
+  int min_chunk;    // units a warp takes at least
+  int q_vec;        // q's rows are 16-byte aligned
+  float* partial;   // pieces [CTAs][2] of items cut by a CTA boundary
   int* meta;        // [CTAs][4]: the item CTA c leaves unfinished {sequence, item, last CTA, 1}, or {.., 0}
   int* status;
 };
@@ -172,9 +178,28 @@ __device__ __forceinline__ void split_unpack(uint32_t w, float* lo, float* hi) {
   }
 }
 
-// Cache lines are read once per item: past L1.
-template <int BYTES>
-__device__ __forceinline__ void split_load(uint32_t* r, const void* p) {
+// BYTES from global to this lane's shared memory, or zeros (FULL: never zeros).
+template <int BYTES, bool FULL>
+__device__ __forceinline__ void split_copy(uint32_t dst, const void* src, bool on) {
+  const int n = on ? BYTES : 0;
+  if constexpr (FULL && BYTES == 16)
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else if constexpr (FULL)
+    asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+  else if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
+                 : "memory");
+}
+// The same to registers; lines are read once per item, past L1.
+template <int BYTES, bool FULL>
+__device__ __forceinline__ void split_load(uint32_t* r, const void* p, bool on) {
+  if constexpr (!FULL) {
+#pragma unroll
+    for (int x = 0; x < BYTES / 4; ++x) r[x] = 0u;
+    if (!on) return;
+  }
   if constexpr (BYTES == 16)
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -183,6 +208,27 @@ __device__ __forceinline__ void split_load(uint32_t* r, const void* p) {
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
   else
     asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+}
+__device__ __forceinline__ void split_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void split_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void split_lds(uint32_t* r, const char* p) {
+  if constexpr (BYTES == 16) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    r[0] = x.x;
+    r[1] = x.y;
+    r[2] = x.z;
+    r[3] = x.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    r[0] = x.x;
+    r[1] = x.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
 }
 
 // ---- shapes of a kind -------------------------------------------------------
@@ -214,6 +260,21 @@ struct SplitCfg {
   static constexpr int kPieceFloats = kRegs * 32;
 };
 
+// A warp's shared memory: fp32 caches keep a ring of tiles there (8-bit and
+// bf16 ones are loaded to registers, which took 20% less time than copying them
+// to shared memory first); the tiles' places and scales; fp32 query rows.
+template <int KIND, int E>
+struct SplitRing {
+  static constexpr bool kRing = KIND == kSplitF32;
+  static constexpr int kSide = kSplitTile * E * SplitCfg<KIND, E>::ES;  // bytes of a tile's K (V)
+  static constexpr int kStages =
+      !kRing ? 1 : (2 * kSide * 8 <= kSplitRing ? 8 : (2 * kSide <= kSplitRing ? kSplitRing / (2 * kSide) : 1));
+  static constexpr int kMetaAt = kRing ? kStages * 2 * kSide : 0;
+  static constexpr int kScaleAt = kMetaAt + kSplitMeta * 16;
+  static constexpr int kQueryAt = kScaleAt + kSplitMeta * 8;
+  static constexpr int kWarpBytes = kQueryAt + (KIND == kSplitF32 ? 8 * E * 4 : 0);
+};
+
 // (m, l, O) of up to 8 query rows over some tiles; columns 2t and 2t + 1 in lane (g, t).
 template <int NM>
 struct SplitState {
@@ -222,18 +283,22 @@ struct SplitState {
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int j = 0; j < NM; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      m[x] = -INFINITY;
+      l[x] = 0.f;
+    }
   }
   __device__ __forceinline__ void put(float* piece, int lane) const {
 #pragma unroll
     for (int j = 0; j < NM; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) piece[(4 * j + r) * 32 + lane] = o[j][r];
-    piece[(4 * NM + 0) * 32 + lane] = m[0];
-    piece[(4 * NM + 1) * 32 + lane] = m[1];
-    piece[(4 * NM + 2) * 32 + lane] = l[0];
-    piece[(4 * NM + 3) * 32 + lane] = l[1];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      piece[(4 * NM + x) * 32 + lane] = m[x];
+      piece[(4 * NM + 2 + x) * 32 + lane] = l[x];
+    }
   }
   // joins the tiles of `piece` (which follow this state's)
   __device__ __forceinline__ void join(const float* piece, int lane) {
@@ -280,34 +345,209 @@ __device__ __forceinline__ void split_write(const SplitParams& p, const SplitSta
       else
         *reinterpret_cast<float2*>(out + d) = make_float2(a, b);
     }
-    if (p.lse && g == 0) p.lse[h] = l == 0.f ? -INFINITY : (st.m[x] + log2f(l)) * 0.69314718055994531f;
+    if (p.lse && g == 0) p.lse[h] = l == 0.f ? -INFINITY : (st.m[x] + (log2f(l) - kUp)) * 0.69314718055994531f;
   }
 }
 
 // ---- a warp's tiles ---------------------------------------------------------
-// One tile's place: its block, rows inside the page, and which keys count.
-struct SplitTile {
-  const char* k;
-  const char* v;
-  uint32_t mask;  // bit j: key j of the tile is seen (0: the tile is skipped)
-  float sk, sv;
+// What a tile's place says: the byte offset of its (block, head) page, the
+// tile's first token in the page, and which keys count.
+struct SplitPlace {
+  long long page;
+  int off;
+  uint32_t mask;  // bit j: key j is seen (none: the tile is skipped); bit 16: the item's last tile
+};
+
+// What every kind of warp shares: the places of its tiles and the walk over them.
+template <int KIND, typename QT, int E>
+struct SplitWalk {
+  using C = SplitCfg<KIND, E>;
+  using R = SplitRing<KIND, E>;
+  static constexpr int S = R::kStages;
+  SplitState<E / 16> st;
+  char* sm;  // this warp's shared memory
+  int lane;
+
+  // ---- places, 32 at a time: lane l has tile l of the next 32, which start at
+  // tile v0 of item ih0 of sequence i0.
+  int i0, ih0, v0;
+  int left;  // tiles from there on
+  int m_id, m_kvh, m_off;
+  uint32_t m_mask;
+
+  // the lane's tile, and its block id
+  __device__ __forceinline__ void place_begin(const SplitParams& p, const int* prefix) {
+    m_id = -1;
+    m_mask = 0u;
+    int i = i0, ih = ih0, v = v0;
+    if (lane < left) {
+      int rem = lane;
+      int nt = prefix[i + 1] - prefix[i];
+      for (;;) {
+        const long long here = (long long)(p.IH - ih) * nt - v;  // tiles the sequence still has
+        if (rem < here) break;
+        rem -= (int)here;
+        ++i;
+        ih = v = 0;
+        nt = prefix[i + 1] - prefix[i];
+      }
+      v += rem;
+      if (v >= nt) {
+        const int d = v / nt;
+        ih += d;
+        v -= d * nt;
+      }
+      const SplitSeq sq = split_seq(p, i);
+      const int r = v < sq.ts ? v : v + sq.skip;
+      const int tpp = p.page / kSplitTile, pg = r / tpp;
+      const int t0 = r * kSplitTile;
+      m_off = (r - pg * tpp) * kSplitTile;
+      m_kvh = ih / p.NRG;
+      m_id = __ldg(p.page_table + (long long)i * p.pt_stride + pg);
+      // keys [0, L - t0) that are first tokens or in the window
+      const int top = min(kSplitTile, sq.L - t0);
+      uint32_t mask = (1u << top) - 1u;
+      if (sq.low > t0) {
+        const int lo = min(kSplitTile, sq.low - t0), first = max(0, min(kSplitTile, p.sinks - t0));
+        mask &= ~((1u << lo) - 1u) | ((1u << first) - 1u);
+      }
+      m_mask = mask | (v == nt - 1 ? 1u << 16 : 0u);
+      if (v == 0) {  // an item starts here: its query rows will be wanted
+        const char* row = reinterpret_cast<const char*>(static_cast<const QT*>(p.q) + (long long)i * p.q_stride +
+                                                        ((long long)m_kvh * p.G + (ih - m_kvh * p.NRG) * 8) * E);
+        const int bytes = min(8, p.G - (ih - m_kvh * p.NRG) * 8) * E * (int)sizeof(QT);
+        for (int x = 0; x < bytes; x += 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(row + x));
+      }
+      ++v;
+      if (v == nt) {
+        v = 0;
+        ++ih;
+      }
+    }
+    // the next ones start behind lane 31's tile
+    i0 = __shfl_sync(0xffffffffu, i, 31);
+    ih0 = __shfl_sync(0xffffffffu, ih, 31);
+    v0 = __shfl_sync(0xffffffffu, v, 31);
+    left -= 32;
+  }
+  // its scales
+  float m_sk, m_sv;
+  __device__ __forceinline__ void place_scales(const SplitParams& p) {
+    m_sk = m_sv = 0.f;
+    if (m_mask & 0xffffu) {
+      if (m_id < 0 || m_id >= p.num_blocks) {
+        if (p.status) atomicOr(p.status, CA_STATUS_TABLE);
+        m_mask &= ~0xffffu;
+      } else if constexpr (C::k8) {
+        m_sk = __ldg(p.ks + (long long)m_id * p.Hk + m_kvh);
+        m_sv = __ldg(p.vs + (long long)m_id * p.Hk + m_kvh);
+      }
+    }
+  }
+  // all of it to shared memory, as the tiles from `base` on
+  __device__ __forceinline__ void place_store(const SplitParams& p, int base) {
+    const int slot = (base + lane) & (kSplitMeta - 1);
+    SplitPlace a;
+    a.page = ((long long)max(m_id, 0) * p.Hk + m_kvh) * (long long)p.page * E * C::ES;
+    a.off = m_off;
+    a.mask = m_mask;
+    if (!(m_mask & 0xffffu)) a.page = a.off = 0;
+    *reinterpret_cast<float2*>(sm + R::kScaleAt + slot * 8) = make_float2(m_sk, m_sv);
+    *reinterpret_cast<int4*>(sm + R::kMetaAt + slot * 16) = *reinterpret_cast<const int4*>(&a);
+    __syncwarp();
+  }
+  __device__ __forceinline__ SplitPlace place(int n) const {
+    const int4 x = *reinterpret_cast<const int4*>(sm + R::kMetaAt + (n & (kSplitMeta - 1)) * 16);
+    return *reinterpret_cast<const SplitPlace*>(&x);
+  }
+  __device__ __forceinline__ char* slot(int n) const { return sm + (n % S) * 2 * R::kSide; }
+
+  // The warp's n tiles, from tile v of item ih of sequence i on, on W (this).
+  // `done` is called with each item's state: done(i, ih, starts, ends).
+  template <typename W, typename F>
+  __device__ __forceinline__ void run(W& w, const SplitParams& p, const int* prefix, int i, int ih, int v, int n,
+                                      F done) {
+    constexpr int kBatch = 32;
+    i0 = i;
+    ih0 = ih;
+    v0 = v;
+    left = n;
+    m_kvh = m_off = 0;
+    place_begin(p, prefix);
+    place_scales(p);
+    place_store(p, 0);
+    bool starts = v == 0;
+#pragma unroll
+    for (int x = 0; x < S; ++x) {
+      if (x < n) w.copy_k(p, x);
+      split_commit();
+      if (x < n) w.copy_v(p, x);
+      split_commit();
+    }
+    for (int x = S; x < min(n, kSplitAhead); ++x) w.ahead(p, x);
+    w.load_q(p, i, ih);
+    w.clear();
+    for (int j = 0; j < n; ++j) {
+      // the next places, in three steps so that no load is waited for (the
+      // ring runs S <= 8 tiles ahead)
+      const int phase = j & (kBatch - 1);
+      if (j - phase + kBatch < n) {
+        if (phase == 0) place_begin(p, prefix);
+        if (phase == kBatch / 4) place_scales(p);
+        if (phase == kBatch / 2) place_store(p, j + kBatch / 2);
+      }
+      const bool ends = w.step(p, j, n);
+      if (ends || j == n - 1) {
+        w.finish();
+        done(i, ih, starts, ends);
+        if (j < n - 1) {
+          if (++ih == p.IH) {
+            ih = 0;
+            do ++i;
+            while (prefix[i + 1] == prefix[i]);
+          }
+          starts = true;
+          w.load_q(p, i, ih);
+          w.clear();
+        }
+      }
+    }
+  }
 };
 
 template <int KIND, typename QT, int E>
-struct SplitWarp {
+struct SplitWarp : SplitWalk<KIND, QT, E> {
   using C = SplitCfg<KIND, E>;
+  using Walk = SplitWalk<KIND, QT, E>;
+  using R = typename Walk::R;
+  using Walk::lane;
+  using Walk::place;
+  using Walk::slot;
+  using Walk::sm;
+  using Walk::st;
   static constexpr bool kPBf16 = KIND == kSplitBf16;                       // operand type of the MMAs
   static constexpr int NQ = KIND == kSplitE4m3 && sizeof(QT) == 4 ? 2 : 1;  // values q is split into
   static constexpr int NP = KIND == kSplitE4m3 && sizeof(QT) == 2 ? 1 : 2;  // values P is split into
-  SplitState<C::NM> st;
-  uint32_t q[NQ][C::NM][2];
+  static constexpr int S = Walk::S;
+  // bf16 outputs: the tensor core adds the tiles up (fp32 outputs add them with FMAs, which round)
+  static constexpr bool kDirect = sizeof(QT) == 2;
+  uint32_t q[KIND == kSplitF32 ? 1 : NQ][KIND == kSplitF32 ? 1 : C::NM][2];
   float qc[2];  // per column: what turns S into log2 units (but for the block's scale)
-  uint32_t kr[KIND == kSplitF32 ? 1 : (C::k8 ? 2 * C::KC * (C::KB / 4) : 4 * C::NM)];
-  uint32_t vr[KIND == kSplitF32 ? 1 : 4][KIND == kSplitF32 ? 1 : C::RUNS * (C::RUNB / 4)];
+  float up[2];  // kUp - m per column; +inf before there is an m
+  float unit, inv_unit;  // 8-bit caches, kDirect: what O is in units of
+  uint32_t kr[R::kRing ? 1 : (C::k8 ? 2 : 4) * C::NM];                    // the next tile's K
+  uint32_t vr[R::kRing ? 1 : 4][R::kRing ? 1 : C::RUNS * (C::RUNB / 4)];  // and V
+
+  __device__ __forceinline__ void clear() {
+    st.clear();
+    up[0] = up[1] = INFINITY;
+    unit = inv_unit = 1.f;
+  }
 
   // The B fragments of Q^T: column g is query row r0 + g of the item.
-  __device__ __forceinline__ void load_q(const SplitParams& p, int i, int kvh, int r0, int lane, float* sq) {
+  __device__ __forceinline__ void load_q(const SplitParams& p, int i, int ih) {
     const int g = lane >> 2, t = lane & 3;
+    const int kvh = ih / p.NRG, r0 = (ih - kvh * p.NRG) * 8;
     const bool have = r0 + g < p.G;
     const QT* src = static_cast<const QT*>(p.q) + (long long)i * p.q_stride + ((long long)kvh * p.G + r0 + g) * E;
     if constexpr (KIND == kSplitBf16) {
@@ -316,21 +556,43 @@ struct SplitWarp {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const int d = 16 * kk + 8 * b + 2 * t;
-          const float lo = have ? to_f32(src[d]) : 0.f, hi = have ? to_f32(src[d + 1]) : 0.f;
-          q[0][kk][b] = split_pack<true>(lo, hi);
+          if (p.q_vec) {
+            q[0][kk][b] = have ? __ldg(reinterpret_cast<const uint32_t*>(src + d)) : 0u;
+          } else {
+            const float lo = have ? to_f32(src[d]) : 0.f, hi = have ? to_f32(src[d + 1]) : 0.f;
+            q[0][kk][b] = split_pack<true>(lo, hi);
+          }
         }
       qc[0] = qc[1] = p.c;
     } else if constexpr (KIND == kSplitE4m3) {
       float x[4 * C::NM];
+      // the lane's dims: KC runs of KB contiguous ones
+#pragma unroll
+      for (int c = 0; c < C::KC; ++c) {
+        const QT* run = src + c * 4 * C::KB + t * C::KB;
+        if (p.q_vec && have) {
+#pragma unroll
+          for (int w = 0; w < C::KB * (int)sizeof(QT) / 16; ++w) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(run) + w);
+            const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              if constexpr (sizeof(QT) == 2) {
+                x[c * C::KB + 8 * w + 2 * y] = bf16_lo(r[y]);
+                x[c * C::KB + 8 * w + 2 * y + 1] = bf16_hi(r[y]);
+              } else {
+                x[c * C::KB + 4 * w + y] = __uint_as_float(r[y]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < C::KB; ++e) x[c * C::KB + e] = have ? to_f32(run[e]) : 0.f;
+        }
+      }
       float top = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < C::NM; ++kk)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = (kk / (C::KB / 4)) * 4 * C::KB + t * C::KB + 4 * (kk % (C::KB / 4)) + e;
-          x[4 * kk + e] = have ? to_f32(src[d]) : 0.f;
-          top = fmaxf(top, fabsf(x[4 * kk + e]));
-        }
+      for (int e = 0; e < 4 * C::NM; ++e) top = fmaxf(top, fabsf(x[e]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // the row's largest value to [2^13, 2^14): f16 then holds a bf16 row to
@@ -357,6 +619,7 @@ struct SplitWarp {
       qc[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
     } else {
       // fp32 caches: the rows go to shared memory, [dim][8]
+      float* sq = reinterpret_cast<float*>(sm + R::kQueryAt);
       __syncwarp();
       for (int x = lane; x < 8 * E; x += 32) {
         const int r = x / E, d = x - r * E;
@@ -370,71 +633,97 @@ struct SplitWarp {
     }
   }
 
-  // Keys that do not count are not read: zero there (never NaN times 0).
-  __device__ __forceinline__ void load_k(const SplitTile& a, int page, int lane) {
+  // ---- a tile's K and V: to registers, or (fp32) into the ring. Keys that do
+  // not count are zeros there, never NaN times 0.
+  __device__ __forceinline__ void copy_k(const SplitParams& p, int n) {
+    const SplitPlace a = place(n);
+    if ((a.mask & 0xffffu) == 0xffffu)
+      copy_k_of<true>(p, a, slot(n));
+    else
+      copy_k_of<false>(p, a, slot(n));
+  }
+  __device__ __forceinline__ void copy_v(const SplitParams& p, int n) {
+    const SplitPlace a = place(n);
+    if ((a.mask & 0xffffu) == 0xffffu)
+      copy_v_of<true>(p, a, slot(n) + R::kSide);
+    else
+      copy_v_of<false>(p, a, slot(n) + R::kSide);
+  }
+  template <bool FULL>
+  __device__ __forceinline__ void copy_k_of(const SplitParams& p, const SplitPlace& a, char* ring) {
     const int g = lane >> 2, t = lane & 3;
+    const char* src = static_cast<const char*>(p.kc) + a.page;
     if constexpr (C::k8) {
+      src += a.off * E + C::skey(0, g) * E + t * C::KB;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int key = C::skey(half, g);
-        const bool on = (a.mask >> key) & 1;
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int c = 0; c < C::KC; ++c) {
-          uint32_t* r = kr + (half * C::KC + c) * (C::KB / 4);
+        for (int c = 0; c < C::KC; ++c)
+          split_load<C::KB, FULL>(kr + (half * C::KC + c) * (C::KB / 4), src + half * 8 * E + c * 4 * C::KB,
+                                  (a.mask >> C::skey(half, g)) & 1);
+    } else {
+      // a pair of keys of dim pair (bf16) or dim (fp32) d
+      src += (a.off + 2 * g) * 4 + (long long)t * p.page * 4;
+      const bool on = (a.mask >> (2 * g)) & 3;
+      const long long step = 16LL * p.page;
+      if constexpr (C::kBf16) {
 #pragma unroll
-          for (int w = 0; w < C::KB / 4; ++w) r[w] = 0u;
-          if (on) split_load<C::KB>(r, a.k + key * E + c * 4 * C::KB + t * C::KB);
+        for (int x = 0; x < 2 * C::NM; ++x) {
+          split_load<8, FULL>(kr + 2 * x, src + x * step, on);
+          if constexpr (!FULL) {  // one of the pair may not count
+            if (!((a.mask >> (2 * g)) & 1)) kr[2 * x] = 0u;
+            if (!((a.mask >> (2 * g + 1)) & 1)) kr[2 * x + 1] = 0u;
+          }
         }
+      } else {
+        const uint32_t dst = smem_u32(ring) + lane * 8;
+#pragma unroll
+        for (int x = 0; x < E / 4; ++x) split_copy<8, FULL>(dst + x * 256, src + x * step, on);
       }
-    } else if constexpr (KIND == kSplitBf16) {
-      const bool on0 = (a.mask >> (2 * g)) & 1, on1 = (a.mask >> (2 * g + 1)) & 1;
-#pragma unroll
-      for (int kk = 0; kk < C::NM; ++kk)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          uint32_t* r = kr + (2 * kk + b) * 2;
-          r[0] = r[1] = 0u;
-          if (on0 || on1) split_load<8>(r, a.k + ((long long)(8 * kk + 4 * b + t) * page + 2 * g) * 4);
-          if (!on0) r[0] = 0u;
-          if (!on1) r[1] = 0u;
-        }
     }
   }
-  __device__ __forceinline__ void load_v(const SplitTile& a, int lane) {
-    if constexpr (KIND != kSplitF32) {
-      const int g = lane >> 2, t = lane & 3;
+  template <bool FULL>
+  __device__ __forceinline__ void copy_v_of(const SplitParams& p, const SplitPlace& a, char* ring) {
+    const int g = lane >> 2, t = lane & 3;
+    const char* src = static_cast<const char*>(p.vc) + a.page + (long long)a.off * E * C::ES;
+    if constexpr (C::kF32) {
+      // every lane reads all of V there: the slot has been read by now
+      __syncwarp();
+      const uint32_t dst = smem_u32(ring);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = C::vkey(x, t);
-        const bool on = (a.mask >> key) & 1;
-#pragma unroll
-        for (int r = 0; r < C::RUNS; ++r) {
-          uint32_t* w = vr[x] + r * (C::RUNB / 4);
-#pragma unroll
-          for (int y = 0; y < C::RUNB / 4; ++y) w[y] = 0u;
-          if (on) split_load<C::RUNB>(w, a.v + ((long long)key * E + r * 8 * C::RL + g * C::RL) * C::ES);
-        }
+      for (int x = 0; x < R::kSide / 512; ++x) {
+        const int at = x * 512 + lane * 16;
+        split_copy<16, FULL>(dst + at, src + at, (a.mask >> (at / (E * 4))) & 1);
       }
+    } else {
+      src += (C::vkey(0, t) * E + g * C::RL) * C::ES;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int r = 0; r < C::RUNS; ++r)
+          split_load<C::RUNB, FULL>(vr[x] + r * (C::RUNB / 4), src + (C::vkey(x, 0) * E + r * 8 * C::RL) * C::ES,
+                                    (a.mask >> C::vkey(x, t)) & 1);
     }
   }
 
   // S^T of the tile: s[0], s[1] = key row g of columns 2t, 2t+1; s[2], s[3] = row g + 8.
-  __device__ __forceinline__ void scores(float (&s)[4], const SplitTile& a, int page, int lane, const float* sq) {
+  __device__ __forceinline__ void scores(float (&s)[4], const char* ks, uint32_t mask) {
     if constexpr (KIND == kSplitF32) {
       // lane (g, t): keys 2g, 2g+1, every 4th dim, all 8 columns; then the t
       // lanes' sums are added so that each keeps its two columns
       const int g = lane >> 2, t = lane & 3;
+      const float* sq = reinterpret_cast<const float*>(sm + R::kQueryAt);
       float acc[2][8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[0][c] = acc[1][c] = 0.f;
-      const bool on0 = (a.mask >> (2 * g)) & 1, on1 = (a.mask >> (2 * g + 1)) & 1;
+      const bool on0 = (mask >> (2 * g)) & 1, on1 = (mask >> (2 * g + 1)) & 1;
 #pragma unroll 8
-      for (int d = t; d < E; d += 4) {
-        uint32_t r[2] = {0u, 0u};
-        if (on0 || on1) split_load<8>(r, a.k + ((long long)d * page + 2 * g) * 4);
+      for (int x = 0; x < E / 4; ++x) {
+        uint32_t r[2];
+        split_lds<8>(r, ks + (x * 32 + lane) * 8);
         const float k0 = on0 ? __uint_as_float(r[0]) : 0.f, k1 = on1 ? __uint_as_float(r[1]) : 0.f;
-        const float4 qa = *reinterpret_cast<const float4*>(sq + d * 8);
-        const float4 qb = *reinterpret_cast<const float4*>(sq + d * 8 + 4);
+        const float4 qa = *reinterpret_cast<const float4*>(sq + (4 * x + t) * 8);
+        const float4 qb = *reinterpret_cast<const float4*>(sq + (4 * x + t) * 8 + 4);
         const float qq[8] = {qa.x, qa.y, qa.z, qa.w, qb.x, qb.y, qb.z, qb.w};
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -467,7 +756,7 @@ struct SplitWarp {
       for (int kk = 0; kk < C::NM; ++kk) {
         uint32_t f[4];
         if constexpr (C::k8) {
-          const uint32_t w0 = kr[kk], w1 = kr[C::KC * (C::KB / 4) + kk];
+          const uint32_t w0 = kr[kk], w1 = kr[C::NM + kk];
           f[0] = f16x2_of_e4m3x2(w0);
           f[1] = f16x2_of_e4m3x2(w1);
           f[2] = f16x2_of_e4m3x2_hi(w0);
@@ -486,59 +775,87 @@ struct SplitWarp {
     }
   }
 
-  // Adds the tile: s as scores() left it.
-  __device__ __forceinline__ void softmax(float (&s)[4], const SplitTile& a, int lane, float (&f)[2]) {
-    const int g = lane >> 2;
-    const bool on0 = (a.mask >> C::skey(0, g)) & 1, on1 = (a.mask >> C::skey(1, g)) & 1;
-    float mt[2], alpha[2];
+  // The tile's weights 2^(x - m + kUp) (s), m the column's reference, and
+  // what they are multiplied by for the values (f).
+  __device__ __forceinline__ void softmax(float (&s)[4], uint32_t mask, float sk, float sv, float& f) {
+    const float c[2] = {C::k8 ? qc[0] * sk : qc[0], C::k8 ? qc[1] * sk : qc[1]};
+    float x[4];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float c = C::k8 ? qc[x] * a.sk : qc[x];
-      s[x] = on0 ? s[x] * c : -INFINITY;
-      s[2 + x] = on1 ? s[2 + x] * c : -INFINITY;
-      mt[x] = fmaxf(s[x], s[2 + x]);
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(s[r], c[r & 1], up[r & 1]);
+    if ((mask & 0xffffu) != 0xffffu) {
+      const int g = lane >> 2;
+      const bool on0 = (mask >> C::skey(0, g)) & 1, on1 = (mask >> C::skey(1, g)) & 1;
+      x[0] = on0 ? x[0] : -INFINITY;
+      x[1] = on0 ? x[1] : -INFINITY;
+      x[2] = on1 ? x[2] : -INFINITY;
+      x[3] = on1 ? x[3] : -INFINITY;
     }
+    // a weight past 2^(kUp + kSlack) (or one that is no number, as all are
+    // before a column has a reference) moves the references
+    if (__any_sync(0xffffffffu, !(fmaxf(x[0], x[2]) <= kUp + kSlack && fmaxf(x[1], x[3]) <= kUp + kSlack))) {
+      const int g = lane >> 2;
+      const bool on0 = (mask >> C::skey(0, g)) & 1, on1 = (mask >> C::skey(1, g)) & 1;
+      float alpha[2];
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      mt[0] = fmaxf(mt[0], __shfl_xor_sync(0xffffffffu, mt[0], o));
-      mt[1] = fmaxf(mt[1], __shfl_xor_sync(0xffffffffu, mt[1], o));
-    }
+      for (int y = 0; y < 2; ++y) {
+        x[y] = on0 ? s[y] * c[y] : -INFINITY;
+        x[2 + y] = on1 ? s[2 + y] * c[y] : -INFINITY;
+        float mt = fmaxf(x[y], x[2 + y]);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float mn = fmaxf(st.m[x], mt[x]);
-      const float mu = mn == -INFINITY ? 0.f : mn, tu = mt[x] == -INFINITY ? 0.f : mt[x];
-      alpha[x] = exp2_approx(st.m[x] - mu);
-      const float beta = exp2_approx(mt[x] - mu);  // the tile's weights are taken against its own maximum
-      s[x] = exp2_approx(s[x] - tu);
-      s[2 + x] = exp2_approx(s[2 + x] - tu);
-      st.l[x] = st.l[x] * alpha[x] + (s[x] + s[2 + x]) * beta;
-      f[x] = C::k8 ? beta * a.sv : beta;
-      if (mt[x] == -INFINITY) f[x] = 0.f;
-      st.m[x] = mn;
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+        for (int o = 4; o < 32; o <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+        const float mn = fmaxf(st.m[y], mt);
+        const float mu = mn == -INFINITY ? 0.f : mn;
+        alpha[y] = exp2_approx(st.m[y] - mu);
+        st.l[y] *= alpha[y];
+        st.m[y] = mn;
+        up[y] = kUp - mn;  // (still no reference: +inf)
+        x[y] = x[y] - mu + kUp;
+        x[2 + y] = x[2 + y] - mu + kUp;
+      }
 #pragma unroll
       for (int j = 0; j < C::NM; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) st.o[j][r] *= alpha[r & 1];
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = exp2_approx(x[r]);
+    st.l[0] += s[0] + s[2];
+    st.l[1] += s[1] + s[3];
+    if constexpr (!C::k8) {
+      f = 1.f;
+    } else if constexpr (!kDirect) {
+      f = sv;
+    } else {
+      // O is kept in units of `unit`: f = sv / unit enters the weights, so it
+      // must neither overflow f16 nor leave its normal range
+      f = sv * inv_unit;
+      if (!(fabsf(f) <= 1.f && fabsf(f) >= 0x1p-16f) && sv != 0.f) {  // (uniform)
+        const float now = fabsf(sv);
+        const float move = unit / now;
+#pragma unroll
+        for (int j = 0; j < C::NM; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st.o[j][r] *= move;
+        unit = now;
+        inv_unit = 1.f / now;
+        f = sv > 0.f ? 1.f : (sv < 0.f ? -1.f : sv);
+      }
+    }
   }
 
   // O += f * (P V), P = s
-  __device__ __forceinline__ void values(const float (&s)[4], const float (&f)[2], const SplitTile& a, int lane) {
+  __device__ __forceinline__ void values(float (&s)[4], float f, const char* vs) {
     if constexpr (KIND == kSplitF32) {
       const int g = lane >> 2, t = lane & 3;
-      const float p0[2] = {s[0] * f[0], s[1] * f[1]}, p1[2] = {s[2] * f[0], s[3] * f[1]};
 #pragma unroll 4
       for (int key = 0; key < 16; ++key) {
         const int from = (key >> 1) * 4 + t;
-        const float w0 = __shfl_sync(0xffffffffu, (key & 1) ? p1[0] : p0[0], from);
-        const float w1 = __shfl_sync(0xffffffffu, (key & 1) ? p1[1] : p0[1], from);
-        if (!((a.mask >> key) & 1)) continue;  // (uniform)
+        const float w0 = __shfl_sync(0xffffffffu, (key & 1) ? s[2] : s[0], from);
+        const float w1 = __shfl_sync(0xffffffffu, (key & 1) ? s[3] : s[1], from);
 #pragma unroll
         for (int r = 0; r < C::RUNS; ++r) {
           uint32_t w[4];
-          split_load<16>(w, a.v + ((long long)key * E + r * 32 + g * 4) * 4);
+          split_lds<16>(w, vs + (key * E + r * 32 + g * 4) * 4);
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             float* o = st.o[2 * r + (y >> 1)];
@@ -548,6 +865,10 @@ struct SplitWarp {
         }
       }
     } else {
+      if constexpr (C::k8 && kDirect) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] *= f;
+      }
       uint32_t b[NP][2];
       b[0][0] = split_pack<kPBf16>(s[0], s[1]);
       b[0][1] = split_pack<kPBf16>(s[2], s[3]);
@@ -580,86 +901,62 @@ struct SplitWarp {
           m[2] = __byte_perm(vr[2][j], vr[3][j], 0x5410u);
           m[3] = __byte_perm(vr[2][j], vr[3][j], 0x7632u);
         }
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (kDirect) {
 #pragma unroll
-        for (int x = 0; x < NP; ++x) split_mma<kPBf16>(d, m, b[x][0], b[x][1]);
+          for (int x = 0; x < NP; ++x) split_mma<kPBf16>(st.o[j], m, b[x][0], b[x][1]);
+        } else {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st.o[j][r] = fmaf(f[r & 1], d[r], st.o[j][r]);
+          for (int x = 0; x < NP; ++x) split_mma<kPBf16>(d, m, b[x][0], b[x][1]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st.o[j][r] = fmaf(f, d[r], st.o[j][r]);
+        }
       }
     }
   }
 
-  // Tiles [v, v + n) of item (i, kvh, r0).
-  __device__ __forceinline__ void run(const SplitParams& p, const SplitSeq& sq, int i, int kvh, int r0, int v, int n,
-                                      int lane, float* smq) {
-    st.clear();
-    const int tpp = p.page / kSplitTile;
-    const long long rowbytes = (long long)p.page * E * C::ES;
-    // the block ids (and scales) of 32 tiles at a time, one per lane
-    int id = -1, off = 0, pos = 0;
-    float sk = 0.f, sv = 0.f;
-    auto meta = [&](int b0) {
-      const int j = b0 + lane;
-      id = -1;
-      if (j < n) {
-        const int vt = v + j;
-        const int r = vt < sq.ts ? vt : vt + sq.skip;
-        const int pg = r / tpp;
-        off = (r - pg * tpp) * kSplitTile;
-        pos = r * kSplitTile;
-        id = __ldg(p.page_table + (long long)i * p.pt_stride + pg);
-        if (id < 0 || id >= p.num_blocks) {
-          if (p.status) atomicOr(p.status, CA_STATUS_TABLE);
-          id = -1;
-        } else if constexpr (C::k8) {
-          sk = __ldg(p.ks + (long long)id * p.Hk + kvh);
-          sv = __ldg(p.vs + (long long)id * p.Hk + kvh);
-        }
+  // Tile j's lines to L2, ahead of the loads (8-bit caches: 16 rows of K and of V
+  // are one run of bytes each).
+  __device__ __forceinline__ void ahead(const SplitParams& p, int j) const {
+    if constexpr (C::k8 && kSplitAhead > S) {
+      if (lane < 2) {
+        const SplitPlace a = place(j);
+        if (a.mask & 0xffffu)
+          bulk_prefetch_l2(static_cast<const char*>(lane ? p.vc : p.kc) + a.page + (long long)a.off * E, 16 * E);
       }
-    };
-    auto tile = [&](int j) {  // tile j of the 32
-      SplitTile a;
-      const int b = __shfl_sync(0xffffffffu, id, j), o = __shfl_sync(0xffffffffu, off, j),
-                t0 = __shfl_sync(0xffffffffu, pos, j);
-      a.sk = __shfl_sync(0xffffffffu, sk, j);
-      a.sv = __shfl_sync(0xffffffffu, sv, j);
-      const long long at = ((long long)max(b, 0) * p.Hk + kvh) * rowbytes;
-      a.k = static_cast<const char*>(p.kc) + at + (long long)o * (C::k8 ? E : 4);
-      a.v = static_cast<const char*>(p.vc) + at + (long long)o * E * C::ES;
-      // keys [0, L - t0) that are first tokens or in the window
-      const int top = min(kSplitTile, sq.L - t0);
-      uint32_t mask = (1u << top) - 1u;
-      if (sq.low > t0) {
-        const int lo = min(kSplitTile, sq.low - t0), first = max(0, min(kSplitTile, p.sinks - t0));
-        mask &= ~((1u << lo) - 1u) | ((1u << first) - 1u);
-      }
-      a.mask = b < 0 ? 0u : mask;
-      return a;
-    };
-    meta(0);
-    SplitTile cur = tile(0);
-    load_q(p, i, kvh, r0, lane, smq);
-    load_k(cur, p.page, lane);
-    load_v(cur, lane);
-    for (int j = 0; j < n; ++j) {
-      SplitTile next = cur;
-      const bool more = j + 1 < n;
-      if (more) {
-        if (((j + 1) & 31) == 0) meta(j + 1);
-        next = tile((j + 1) & 31);
-      }
-      float s[4], f[2];
-      scores(s, cur, p.page, lane, smq);
-      if (more) load_k(next, p.page, lane);
-      softmax(s, cur, lane, f);
-      values(s, f, cur, lane);
-      if (more) load_v(next, lane);
-      cur = next;
     }
+  }
+
+  // Tile j: true when its item ends.
+  __device__ __forceinline__ bool step(const SplitParams& p, int j, int n) {
+    if (j + kSplitAhead < n) ahead(p, j + kSplitAhead);
+    const uint32_t mask = place(j).mask;
+    const float2 sc = *reinterpret_cast<const float2*>(sm + R::kScaleAt + (j & (kSplitMeta - 1)) * 8);
+    char* at = slot(j);
+    float s[4], f;
+    split_wait<2 * S - 1>();
+    scores(s, at, mask);
+    if (j + S < n) copy_k(p, j + S);
+    split_commit();
+    softmax(s, mask, sc.x, sc.y, f);
+    split_wait<2 * S - 1>();
+    if constexpr (C::kF32) __syncwarp();
+    values(s, f, at + R::kSide);
+    if (j + S < n) copy_v(p, j + S);
+    split_commit();
+    return (mask >> 16) & 1;
+  }
+  __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) st.l[x] += __shfl_xor_sync(0xffffffffu, st.l[x], o);
+    if constexpr (C::k8 && kDirect) {
+#pragma unroll
+      for (int x = 0; x < C::NM; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.o[x][r] *= unit;
+    }
   }
 };
 
@@ -672,18 +969,49 @@ struct SplitPiece {
 
 template <int KIND, int E>
 __host__ __device__ constexpr int split_smem_fixed() {
-  return kSplitWarps * 2 * SplitCfg<KIND, E>::kPieceFloats * 4 + kSplitWarps * 2 * (int)sizeof(SplitPiece) +
-         (KIND == kSplitF32 ? kSplitWarps * 8 * E * 4 : 0) + 128;
+  return kSplitWarps * (SplitRing<KIND, E>::kWarpBytes + 2 * SplitCfg<KIND, E>::kPieceFloats * 4) + kSplitWarps * 2 * (int)sizeof(SplitPiece) + 128;
+}
+
+// Work is shared out in units: an item is kSplitItemUnits and one for each of
+// its tiles. Where unit u of the launch lies: the tile at or after it.
+constexpr int kSplitItemUnits = 2;
+
+struct SplitSpot {
+  int i, ih, v;
+  long long tile;  // its number among the launch's tiles
+};
+__device__ __forceinline__ long long split_units(const int* prefix, int i, int IH) {
+  return ((long long)prefix[i] + (long long)kSplitItemUnits * i) * IH;
+}
+__device__ __forceinline__ SplitSpot split_spot(const int* prefix, int B, int IH, long long u) {
+  int lo = 0, hi = B;  // the last i that starts at or before u
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (split_units(prefix, mid, IH) <= u)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  SplitSpot s;
+  s.i = lo;
+  const int nt = prefix[lo + 1] - prefix[lo];
+  const long long r = u - split_units(prefix, lo, IH);
+  const long long ih = min((long long)IH, r / (nt + kSplitItemUnits));
+  s.ih = (int)ih;
+  s.v = (int)max(0LL, r - ih * (nt + kSplitItemUnits) - kSplitItemUnits);
+  if (s.ih == IH) s.v = 0;  // (u is the end)
+  s.tile = (long long)prefix[lo] * IH + ih * nt + min(s.v, nt);
+  return s;
 }
 
 template <int KIND, typename QT, int E>
 __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
     split_decode_kernel(const __grid_constant__ SplitParams p) {
   using C = SplitCfg<KIND, E>;
+  constexpr int kWarpBytes = SplitRing<KIND, E>::kWarpBytes;
   extern __shared__ __align__(16) char split_smem[];
-  float* pieces = reinterpret_cast<float*>(split_smem);  // [warp][head, tail]
-  float* smq = pieces + kSplitWarps * 2 * C::kPieceFloats;
-  SplitPiece* info = reinterpret_cast<SplitPiece*>(smq + (KIND == kSplitF32 ? kSplitWarps * 8 * E : 0));
+  float* pieces = reinterpret_cast<float*>(split_smem + kSplitWarps * kWarpBytes);  // [warp][head, tail]
+  SplitPiece* info = reinterpret_cast<SplitPiece*>(pieces + kSplitWarps * 2 * C::kPieceFloats);
   int* wsum = reinterpret_cast<int*>(info + kSplitWarps * 2);
   int* prefix = wsum + 32;  // [B + 1]: tiles of one item before sequence i
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -709,12 +1037,34 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
     __syncthreads();
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long total = (long long)prefix[p.B] * p.IH;
+  const long long total = split_units(prefix, p.B, p.IH);
   const long long warps = (long long)gridDim.x * kSplitWarps;
   const long long chunk = max((long long)p.min_chunk, (total + warps - 1) / warps);
-  const long long w0 = ((long long)blockIdx.x * kSplitWarps + warp) * chunk;
+  const long long w0 = min(total, ((long long)blockIdx.x * kSplitWarps + warp) * chunk);
   const long long w1 = min(total, w0 + chunk);
 
+  // ---- this warp's tiles
+  if (w0 < w1) {
+    SplitSpot a = split_spot(prefix, p.B, p.IH, w0);
+    const int n = (int)(split_spot(prefix, p.B, p.IH, w1).tile - a.tile);
+    if (n > 0) {
+      while (prefix[a.i + 1] == prefix[a.i]) {  // sequences that see nothing have no tiles
+        ++a.i;
+        a.ih = a.v = 0;
+      }
+      SplitWarp<KIND, QT, E> w;
+      w.sm = split_smem + warp * kWarpBytes;
+      w.lane = lane;
+      w.run(w, p, prefix, a.i, a.ih, a.v, n, [&](int i, int ih, bool starts, bool ends) {
+        if (starts && ends) {
+          split_write<KIND, QT, E>(p, w.st, i, ih, lane);
+        } else {
+          w.st.put(pieces + (warp * 2 + (starts ? 1 : 0)) * C::kPieceFloats, lane);
+          if (lane == 0) info[warp * 2 + (starts ? 1 : 0)] = SplitPiece{i, ih, ends ? 1 : 0, 1};
+        }
+      });
+    }
+  }
   // ---- sequences that see nothing: zeros
   for (int i = blockIdx.x; i < p.B; i += gridDim.x)
     if (prefix[i + 1] == prefix[i]) {
@@ -723,54 +1073,14 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
       if (p.lse)
         for (int x = threadIdx.x; x < p.H; x += kThreads) p.lse[(long long)i * p.H + x] = -INFINITY;
     }
-
-  // ---- this warp's tiles
-  if (w0 < w1) {
-    const long long u = w0 / p.IH;
-    int lo = 0, hi = p.B;  // the last i with prefix[i] <= u
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= u)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    int i = lo;
-    const int nt0 = prefix[i + 1] - prefix[i];
-    const long long rem = w0 - (long long)prefix[i] * p.IH;
-    int ih = (int)(rem / nt0), v = (int)(rem - (long long)ih * nt0);
-    SplitSeq sq = split_seq(p, i);
-    SplitWarp<KIND, QT, E> w;
-    for (long long at = w0;;) {
-      const int n = (int)min((long long)(sq.nt - v), w1 - at);
-      const int kvh = ih / p.NRG;
-      w.run(p, sq, i, kvh, (ih - kvh * p.NRG) * 8, v, n, lane, smq + warp * 8 * E);
-      const bool starts = v == 0, ends = v + n == sq.nt;
-      if (starts && ends) {
-        split_write<KIND, QT, E>(p, w.st, i, ih, lane);
-      } else {
-        const int slot = warp * 2 + (starts ? 1 : 0);
-        w.st.put(pieces + slot * C::kPieceFloats, lane);
-        if (lane == 0) info[slot] = SplitPiece{i, ih, ends ? 1 : 0, 1};
-      }
-      at += n;
-      if (at >= w1) break;
-      v = 0;
-      if (++ih == p.IH) {
-        ih = 0;
-        do ++i;
-        while (prefix[i + 1] == prefix[i]);
-        sq = split_seq(p, i);
-      }
-    }
-  }
   if (threadIdx.x == 0) p.meta[4 * blockIdx.x + 3] = 0;
   __syncthreads();
 
   // ---- join the pieces of one item inside this CTA, in order. A group starts
-  // with a warp's tail piece (the item's first tile), or with warp 0's head
-  // piece (the item began in an earlier CTA), and goes on through the next
-  // warps' head pieces until the item's last tile or the CTA's end.
+  // with a warp's tail piece (the item's first tile), or with the head piece of
+  // the first warp that has tiles (the item began in an earlier CTA), and goes
+  // on through the next warps' head pieces until the item's last tile or the
+  // CTA's end. (A range that starts inside an item has tiles of it.)
   for (int kind = 0; kind < 2; ++kind) {  // 0: warp 0's head, 1: this warp's tail
     if (kind == 0 && warp != 0) continue;
     const int first = warp * 2 + kind;
@@ -789,9 +1099,9 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
     } else {
       st.put(p.partial + (2LL * blockIdx.x + kind) * C::kPieceFloats, lane);
       if (kind == 1 && lane == 0) {
-        // the item's last tile, and the CTA that holds it
-        const long long end = (long long)prefix[me.i] * p.IH +
-                              (long long)(me.ih + 1) * (prefix[me.i + 1] - prefix[me.i]) - 1;
+        // the CTA that holds the item's last unit (its last tile)
+        const long long end = split_units(prefix, me.i, p.IH) +
+                              (long long)(me.ih + 1) * (prefix[me.i + 1] - prefix[me.i] + kSplitItemUnits) - 1;
         int* m = p.meta + 4 * blockIdx.x;
         m[0] = me.i;
         m[1] = me.ih;
@@ -803,29 +1113,65 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
 }
 
 // Joins the items that cross CTA boundaries: block c takes the one that CTA c
-// began and did not end, if there is one.
+// began and did not end, if there is one. Warp (r, j) joins a contiguous share r
+// of the item's pieces for the four registers j of O (loads of several pieces in
+// flight); then the shares are joined in order.
 template <int KIND, typename QT, int E>
-__global__ void __launch_bounds__(32 * kSplitMergeWarps) split_merge_kernel(const __grid_constant__ SplitParams p) {
+__global__ void __launch_bounds__(32 * kSplitMergeShares * (E / 16))
+    split_merge_kernel(const __grid_constant__ SplitParams p) {
   using C = SplitCfg<KIND, E>;
-  __shared__ float pieces[kSplitMergeWarps * C::kPieceFloats];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float shares[kSplitMergeShares * C::kPieceFloats];
+  const int lane = threadIdx.x & 31;
+  const int j = (threadIdx.x >> 5) % C::NM, share = (threadIdx.x >> 5) / C::NM;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
   const int* m = p.meta + 4 * c;
   if (m[3] != 1) return;
-  const int last = m[2], n = last - c + 1;
-  // warp w joins a contiguous share of the pieces, then warp 0 the shares
-  const int per = (n + kSplitMergeWarps - 1) / kSplitMergeWarps;
-  SplitState<C::NM> st;
+  const int n = m[2] - c + 1;
+  const int per = (n + kSplitMergeShares - 1) / kSplitMergeShares;
+  const int k0 = share * per, k1 = min(n, k0 + per);
+  // one group of four registers, and (m, l) with it
+  SplitState<1> st;
   st.clear();
-  for (int k = warp * per; k < min(n, (warp + 1) * per); ++k)
-    st.join(p.partial + (2LL * (c + k) + (k == 0 ? 1 : 0)) * C::kPieceFloats, lane);
-  st.put(pieces + warp * C::kPieceFloats, lane);
+#pragma unroll 4
+  for (int k = k0; k < k1; ++k) {
+    const float* piece = p.partial + (2LL * (c + k) + (k == 0 ? 1 : 0)) * C::kPieceFloats + lane;
+    float o[4], mo[2], lo[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = piece[(4 * j + r) * 32];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      mo[x] = piece[(4 * C::NM + x) * 32];
+      lo[x] = piece[(4 * C::NM + 2 + x) * 32];
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float mn = fmaxf(st.m[x], mo[x]);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float a = exp2_approx(st.m[x] - mu), b = exp2_approx(mo[x] - mu);
+      st.l[x] = st.l[x] * a + lo[x] * b;
+      st.m[x] = mn;
+      st.o[0][x] = st.o[0][x] * a + o[x] * b;
+      st.o[0][2 + x] = st.o[0][2 + x] * a + o[2 + x] * b;
+    }
+  }
+  float* mine = shares + share * C::kPieceFloats + lane;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) mine[(4 * j + r) * 32] = st.o[0][r];
+  if (j == 0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      mine[(4 * C::NM + x) * 32] = st.m[x];
+      mine[(4 * C::NM + 2 + x) * 32] = st.l[x];
+    }
+  }
   __syncthreads();
-  if (warp == 0) {
+  if (threadIdx.x < 32) {
+    SplitState<C::NM> all;
+    all.clear();
 #pragma unroll 1
-    for (int w = 1; w < kSplitMergeWarps; ++w) st.join(pieces + w * C::kPieceFloats, lane);
-    split_write<KIND, QT, E>(p, st, m[0], m[1], lane);
+    for (int r = 0; r < kSplitMergeShares; ++r) all.join(shares + r * C::kPieceFloats, lane);
+    split_write<KIND, QT, E>(p, all, m[0], m[1], lane);
   }
 }
 
