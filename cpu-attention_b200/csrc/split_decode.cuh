@@ -36,8 +36,8 @@
 //   8-bit codes widen exactly to f16; q is scaled by a power of two per row so
 //   that f16 holds it. P enters as one f16 value for bf16 outputs (2^-12 of the
 //   weight, against 2^-9 of the output's rounding) and as a value plus its rest
-//   for fp32 ones and for bf16 caches; s_v enters with it, against a unit that
-//   follows the scales a user stores (fp32 outputs: when the tile is added).
+//   for fp32 ones and for bf16 caches; s_v enters with it, its exponent with the
+//   weight's, so any scales a user stores are followed.
 // fp32 caches run the same tiles on FMAs.
 //
 // Loads of tile n+1 are issued as soon as the registers of tile n are free: 12
@@ -263,6 +263,13 @@ struct SplitCfg {
 // A warp's shared memory: fp32 caches keep a ring of tiles there (8-bit and
 // bf16 ones are loaded to registers, which took 20% less time than copying them
 // to shared memory first); the tiles' places and scales; fp32 query rows.
+// Groups of 16 tokens a tile has: small heads take several, so that a warp has 4
+// KiB (bf16: 4 KiB or more) in flight whatever the head_dim.
+template <int KIND, int E>
+__host__ __device__ constexpr int split_sub() {
+  return KIND == kSplitE4m3 ? 128 / E : (KIND == kSplitBf16 && E == 32 ? 2 : 1);
+}
+
 template <int KIND, int E>
 struct SplitRing {
   static constexpr bool kRing = KIND == kSplitF32;
@@ -271,7 +278,7 @@ struct SplitRing {
       !kRing ? 1 : (2 * kSide * 8 <= kSplitRing ? 8 : (2 * kSide <= kSplitRing ? kSplitRing / (2 * kSide) : 1));
   static constexpr int kMetaAt = kRing ? kStages * 2 * kSide : 0;
   static constexpr int kScaleAt = kMetaAt + kSplitMeta * 16;
-  static constexpr int kQueryAt = kScaleAt + kSplitMeta * 8;
+  static constexpr int kQueryAt = kScaleAt + (KIND == kSplitE4m3 ? kSplitMeta * 16 : 0);
   static constexpr int kWarpBytes = kQueryAt + (KIND == kSplitF32 ? 8 * E * 4 : 0);
 };
 
@@ -364,12 +371,13 @@ struct SplitWalk {
   using C = SplitCfg<KIND, E>;
   using R = SplitRing<KIND, E>;
   static constexpr int S = R::kStages;
+  static constexpr int SUB = split_sub<KIND, E>();
   SplitState<E / 16> st;
   char* sm;  // this warp's shared memory
   int lane;
 
-  // ---- places, 32 at a time: lane l has tile l of the next 32, which start at
-  // tile v0 of item ih0 of sequence i0.
+  // ---- places, 32 at a time: lane l has the 16 tokens l % SUB of tile l / SUB
+  // of the next 32 / SUB tiles, which start at tile v0 of item ih0 of sequence i0.
   int i0, ih0, v0;
   int left;  // tiles from there on
   int m_id, m_kvh, m_off;
@@ -380,8 +388,8 @@ struct SplitWalk {
     m_id = -1;
     m_mask = 0u;
     int i = i0, ih = ih0, v = v0;
-    if (lane < left) {
-      int rem = lane;
+    if (lane / SUB < left) {
+      int rem = lane / SUB;
       int nt = prefix[i + 1] - prefix[i];
       for (;;) {
         const long long here = (long long)(p.IH - ih) * nt - v;  // tiles the sequence still has
@@ -398,21 +406,24 @@ struct SplitWalk {
         v -= d * nt;
       }
       const SplitSeq sq = split_seq(p, i);
-      const int r = v < sq.ts ? v : v + sq.skip;
-      const int tpp = p.page / kSplitTile, pg = r / tpp;
-      const int t0 = r * kSplitTile;
-      m_off = (r - pg * tpp) * kSplitTile;
+      const int u = v * SUB + lane % SUB;  // of the sequence's groups of 16 tokens
       m_kvh = ih / p.NRG;
-      m_id = __ldg(p.page_table + (long long)i * p.pt_stride + pg);
-      // keys [0, L - t0) that are first tokens or in the window
-      const int top = min(kSplitTile, sq.L - t0);
-      uint32_t mask = (1u << top) - 1u;
-      if (sq.low > t0) {
-        const int lo = min(kSplitTile, sq.low - t0), first = max(0, min(kSplitTile, p.sinks - t0));
-        mask &= ~((1u << lo) - 1u) | ((1u << first) - 1u);
+      if (u < sq.nt) {
+        const int r = u < sq.ts ? u : u + sq.skip;
+        const int tpp = p.page / kSplitTile, pg = r / tpp;
+        const int t0 = r * kSplitTile;
+        m_off = (r - pg * tpp) * kSplitTile;
+        m_id = __ldg(p.page_table + (long long)i * p.pt_stride + pg);
+        // keys [0, L - t0) that are first tokens or in the window
+        const int top = min(kSplitTile, sq.L - t0);
+        m_mask = (1u << top) - 1u;
+        if (sq.low > t0) {
+          const int lo = min(kSplitTile, sq.low - t0), first = max(0, min(kSplitTile, p.sinks - t0));
+          m_mask &= ~((1u << lo) - 1u) | ((1u << first) - 1u);
+        }
       }
-      m_mask = mask | (v == nt - 1 ? 1u << 16 : 0u);
-      if (v == 0) {  // an item starts here: its query rows will be wanted
+      if (v == nt - 1) m_mask |= 1u << 16;
+      if (v == 0 && lane % SUB == 0) {  // an item starts here: its query rows will be wanted
         const char* row = reinterpret_cast<const char*>(static_cast<const QT*>(p.q) + (long long)i * p.q_stride +
                                                         ((long long)m_kvh * p.G + (ih - m_kvh * p.NRG) * 8) * E);
         const int bytes = min(8, p.G - (ih - m_kvh * p.NRG) * 8) * E * (int)sizeof(QT);
@@ -428,7 +439,7 @@ struct SplitWalk {
     i0 = __shfl_sync(0xffffffffu, i, 31);
     ih0 = __shfl_sync(0xffffffffu, ih, 31);
     v0 = __shfl_sync(0xffffffffu, v, 31);
-    left -= 32;
+    left -= 32 / SUB;
   }
   // its scales
   float m_sk, m_sv;
@@ -446,17 +457,22 @@ struct SplitWalk {
   }
   // all of it to shared memory, as the tiles from `base` on
   __device__ __forceinline__ void place_store(const SplitParams& p, int base) {
-    const int slot = (base + lane) & (kSplitMeta - 1);
+    const int slot = (base * SUB + lane) & (kSplitMeta - 1);
     SplitPlace a;
     a.page = ((long long)max(m_id, 0) * p.Hk + m_kvh) * (long long)p.page * E * C::ES;
     a.off = m_off;
     a.mask = m_mask;
     if (!(m_mask & 0xffffu)) a.page = a.off = 0;
-    *reinterpret_cast<float2*>(sm + R::kScaleAt + slot * 8) = make_float2(m_sk, m_sv);
+    if constexpr (C::k8) {
+      // s_v as 2^e * g, 1 <= |g| < 2
+      const int e = m_sv == 0.f ? -1000 : ilogbf(m_sv);
+      const float g = m_sv == 0.f ? 0.f : scalbnf(m_sv, -e);
+      *reinterpret_cast<float4*>(sm + R::kScaleAt + slot * 16) = make_float4(m_sk, (float)e, g, 0.f);
+    }
     *reinterpret_cast<int4*>(sm + R::kMetaAt + slot * 16) = *reinterpret_cast<const int4*>(&a);
     __syncwarp();
   }
-  __device__ __forceinline__ SplitPlace place(int n) const {
+  __device__ __forceinline__ SplitPlace place(int n) const {  // of the 16 tokens n of the stream
     const int4 x = *reinterpret_cast<const int4*>(sm + R::kMetaAt + (n & (kSplitMeta - 1)) * 16);
     return *reinterpret_cast<const SplitPlace*>(&x);
   }
@@ -467,7 +483,7 @@ struct SplitWalk {
   template <typename W, typename F>
   __device__ __forceinline__ void run(W& w, const SplitParams& p, const int* prefix, int i, int ih, int v, int n,
                                       F done) {
-    constexpr int kBatch = 32;
+    constexpr int kBatch = 32 / SUB;
     i0 = i;
     ih0 = ih;
     v0 = v;
@@ -528,20 +544,25 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
   static constexpr bool kPBf16 = KIND == kSplitBf16;                       // operand type of the MMAs
   static constexpr int NQ = KIND == kSplitE4m3 && sizeof(QT) == 4 ? 2 : 1;  // values q is split into
   static constexpr int NP = KIND == kSplitE4m3 && sizeof(QT) == 2 ? 1 : 2;  // values P is split into
-  static constexpr int S = Walk::S;
+  static constexpr int S = Walk::S, SUB = Walk::SUB;
   // bf16 outputs: the tensor core adds the tiles up (fp32 outputs add them with FMAs, which round)
   static constexpr bool kDirect = sizeof(QT) == 2;
   uint32_t q[KIND == kSplitF32 ? 1 : NQ][KIND == kSplitF32 ? 1 : C::NM][2];
   float qc[2];  // per column: what turns S into log2 units (but for the block's scale)
   float up[2];  // kUp - m per column; +inf before there is an m
-  float unit, inv_unit;  // 8-bit caches, kDirect: what O is in units of
-  uint32_t kr[R::kRing ? 1 : (C::k8 ? 2 : 4) * C::NM];                    // the next tile's K
-  uint32_t vr[R::kRing ? 1 : 4][R::kRing ? 1 : C::RUNS * (C::RUNB / 4)];  // and V
+  // 8-bit caches: O is in units of 2^unit, the largest V scale's exponent so far.
+  // A weight times its scale is 2^(x + e - m + kUp) * g, e the scale's exponent
+  // less unit: m follows x + e, so the weights that count most for the values
+  // are near f16's largest whatever the scales. (lift: see follow().)
+  float unit, lift;
+  uint32_t kr[SUB][R::kRing ? 1 : (C::k8 ? 2 : 4) * C::NM];                    // the next tile's K
+  uint32_t vr[SUB][R::kRing ? 1 : 4][R::kRing ? 1 : C::RUNS * (C::RUNB / 4)];  // and V
 
   __device__ __forceinline__ void clear() {
     st.clear();
     up[0] = up[1] = INFINITY;
-    unit = inv_unit = 1.f;
+    unit = -1000.f;
+    lift = 0.f;
   }
 
   // The B fragments of Q^T: column g is query row r0 + g of the item.
@@ -636,21 +657,27 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
   // ---- a tile's K and V: to registers, or (fp32) into the ring. Keys that do
   // not count are zeros there, never NaN times 0.
   __device__ __forceinline__ void copy_k(const SplitParams& p, int n) {
-    const SplitPlace a = place(n);
-    if ((a.mask & 0xffffu) == 0xffffu)
-      copy_k_of<true>(p, a, slot(n));
-    else
-      copy_k_of<false>(p, a, slot(n));
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      const SplitPlace a = place(n * SUB + u);
+      if ((a.mask & 0xffffu) == 0xffffu)
+        copy_k_of<true>(p, a, slot(n), kr[u]);
+      else
+        copy_k_of<false>(p, a, slot(n), kr[u]);
+    }
   }
   __device__ __forceinline__ void copy_v(const SplitParams& p, int n) {
-    const SplitPlace a = place(n);
-    if ((a.mask & 0xffffu) == 0xffffu)
-      copy_v_of<true>(p, a, slot(n) + R::kSide);
-    else
-      copy_v_of<false>(p, a, slot(n) + R::kSide);
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      const SplitPlace a = place(n * SUB + u);
+      if ((a.mask & 0xffffu) == 0xffffu)
+        copy_v_of<true>(p, a, slot(n) + R::kSide, vr[u]);
+      else
+        copy_v_of<false>(p, a, slot(n) + R::kSide, vr[u]);
+    }
   }
-  template <bool FULL>
-  __device__ __forceinline__ void copy_k_of(const SplitParams& p, const SplitPlace& a, char* ring) {
+  template <bool FULL, int N>
+  __device__ __forceinline__ void copy_k_of(const SplitParams& p, const SplitPlace& a, char* ring, uint32_t (&kr)[N]) {
     const int g = lane >> 2, t = lane & 3;
     const char* src = static_cast<const char*>(p.kc) + a.page;
     if constexpr (C::k8) {
@@ -682,8 +709,9 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
       }
     }
   }
-  template <bool FULL>
-  __device__ __forceinline__ void copy_v_of(const SplitParams& p, const SplitPlace& a, char* ring) {
+  template <bool FULL, int N4, int N>
+  __device__ __forceinline__ void copy_v_of(const SplitParams& p, const SplitPlace& a, char* ring,
+                                            uint32_t (&vr)[N4][N]) {
     const int g = lane >> 2, t = lane & 3;
     const char* src = static_cast<const char*>(p.vc) + a.page + (long long)a.off * E * C::ES;
     if constexpr (C::kF32) {
@@ -707,7 +735,8 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
   }
 
   // S^T of the tile: s[0], s[1] = key row g of columns 2t, 2t+1; s[2], s[3] = row g + 8.
-  __device__ __forceinline__ void scores(float (&s)[4], const char* ks, uint32_t mask) {
+  template <int N>
+  __device__ __forceinline__ void scores(float (&s)[4], const char* ks, uint32_t mask, const uint32_t (&kr)[N]) {
     if constexpr (KIND == kSplitF32) {
       // lane (g, t): keys 2g, 2g+1, every 4th dim, all 8 columns; then the t
       // lanes' sums are added so that each keeps its two columns
@@ -775,42 +804,91 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
     }
   }
 
-  // The tile's weights 2^(x - m + kUp) (s), m the column's reference, and
-  // what they are multiplied by for the values (f).
-  __device__ __forceinline__ void softmax(float (&s)[4], uint32_t mask, float sk, float sv, float& f) {
-    const float c[2] = {C::k8 ? qc[0] * sk : qc[0], C::k8 ? qc[1] * sk : qc[1]};
-    float x[4];
+  // A larger V scale than any before: O in its units. Its tokens' weights would
+  // be small against m, which was made with smaller scales: m goes down with
+  // them (l and O up), by 2^90 in all at most, so that l stays finite.
+  __device__ __forceinline__ void follow(float e) {
+    const float d = unit - e;  // < 0
+    const float rise = unit < -500.f ? 0.f : fminf(-d, 90.f - lift);
+    const float fo = unit < -500.f ? 0.f : exp2f(fmaxf(d + rise, -140.f)), fl = exp2f(rise);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = fmaf(s[r], c[r & 1], up[r & 1]);
-    if ((mask & 0xffffu) != 0xffffu) {
-      const int g = lane >> 2;
-      const bool on0 = (mask >> C::skey(0, g)) & 1, on1 = (mask >> C::skey(1, g)) & 1;
-      x[0] = on0 ? x[0] : -INFINITY;
-      x[1] = on0 ? x[1] : -INFINITY;
-      x[2] = on1 ? x[2] : -INFINITY;
-      x[3] = on1 ? x[3] : -INFINITY;
+    for (int j = 0; j < C::NM; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st.o[j][r] *= fo;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      st.l[y] *= fl;
+      st.m[y] -= rise;
+      up[y] += rise;
+    }
+    lift += rise;
+    unit = e;
+  }
+
+  // The tile's weights 2^(x + e - m + kUp) (s), m the column's reference, and
+  // what they are multiplied by for the values (g).
+  __device__ __forceinline__ void softmax(float (&s)[SUB][4], const uint32_t (&mask)[SUB], const float4 (&sc)[SUB],
+                                          float (&gv)[SUB]) {
+    const int g = lane >> 2;
+    float x[SUB][4], e[SUB], back[SUB];  // back: 2^-e, from these weights to those of l
+    bool fits = true;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      e[u] = 0.f;
+      back[u] = gv[u] = 1.f;
+      if constexpr (C::k8)
+        if (sc[u].y > unit) follow(sc[u].y);  // (uniform)
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      if constexpr (C::k8) {
+        const float d = sc[u].y - unit;
+        e[u] = fmaxf(d, -90.f);
+        back[u] = exp2_approx(-e[u]);
+        gv[u] = d >= -90.f ? sc[u].z : sc[u].z * exp2_approx(fmaxf(d, -200.f) + 90.f);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x[u][r] = fmaf(s[u][r], C::k8 ? qc[r & 1] * sc[u].x : qc[r & 1], C::k8 ? up[r & 1] + e[u] : up[r & 1]);
+      if ((mask[u] & 0xffffu) != 0xffffu) {
+        const bool on0 = (mask[u] >> C::skey(0, g)) & 1, on1 = (mask[u] >> C::skey(1, g)) & 1;
+        x[u][0] = on0 ? x[u][0] : -INFINITY;
+        x[u][1] = on0 ? x[u][1] : -INFINITY;
+        x[u][2] = on1 ? x[u][2] : -INFINITY;
+        x[u][3] = on1 ? x[u][3] : -INFINITY;
+      }
+      fits = fits && fmaxf(x[u][0], x[u][2]) <= kUp + kSlack && fmaxf(x[u][1], x[u][3]) <= kUp + kSlack;
     }
     // a weight past 2^(kUp + kSlack) (or one that is no number, as all are
     // before a column has a reference) moves the references
-    if (__any_sync(0xffffffffu, !(fmaxf(x[0], x[2]) <= kUp + kSlack && fmaxf(x[1], x[3]) <= kUp + kSlack))) {
-      const int g = lane >> 2;
-      const bool on0 = (mask >> C::skey(0, g)) & 1, on1 = (mask >> C::skey(1, g)) & 1;
-      float alpha[2];
+    if (__any_sync(0xffffffffu, !fits)) {
+      float mt[2] = {-INFINITY, -INFINITY}, alpha[2];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const bool on0 = (mask[u] >> C::skey(0, g)) & 1, on1 = (mask[u] >> C::skey(1, g)) & 1;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float c = C::k8 ? qc[y] * sc[u].x : qc[y];
+          x[u][y] = on0 ? fmaf(s[u][y], c, e[u]) : -INFINITY;
+          x[u][2 + y] = on1 ? fmaf(s[u][2 + y], c, e[u]) : -INFINITY;
+          mt[y] = fmaxf(mt[y], fmaxf(x[u][y], x[u][2 + y]));
+        }
+      }
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        x[y] = on0 ? s[y] * c[y] : -INFINITY;
-        x[2 + y] = on1 ? s[2 + y] * c[y] : -INFINITY;
-        float mt = fmaxf(x[y], x[2 + y]);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-        const float mn = fmaxf(st.m[y], mt);
+        for (int o = 4; o < 32; o <<= 1) mt[y] = fmaxf(mt[y], __shfl_xor_sync(0xffffffffu, mt[y], o));
+        const float mn = fmaxf(st.m[y], mt[y]);
         const float mu = mn == -INFINITY ? 0.f : mn;
         alpha[y] = exp2_approx(st.m[y] - mu);
         st.l[y] *= alpha[y];
         st.m[y] = mn;
         up[y] = kUp - mn;  // (still no reference: +inf)
-        x[y] = x[y] - mu + kUp;
-        x[2 + y] = x[2 + y] - mu + kUp;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          x[u][y] = x[u][y] - mu + kUp;
+          x[u][2 + y] = x[u][2 + y] - mu + kUp;
+        }
       }
 #pragma unroll
       for (int j = 0; j < C::NM; ++j)
@@ -818,33 +896,17 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
         for (int r = 0; r < 4; ++r) st.o[j][r] *= alpha[r & 1];
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = exp2_approx(x[r]);
-    st.l[0] += s[0] + s[2];
-    st.l[1] += s[1] + s[3];
-    if constexpr (!C::k8) {
-      f = 1.f;
-    } else if constexpr (!kDirect) {
-      f = sv;
-    } else {
-      // O is kept in units of `unit`: f = sv / unit enters the weights, so it
-      // must neither overflow f16 nor leave its normal range
-      f = sv * inv_unit;
-      if (!(fabsf(f) <= 1.f && fabsf(f) >= 0x1p-16f) && sv != 0.f) {  // (uniform)
-        const float now = fabsf(sv);
-        const float move = unit / now;
+    for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-        for (int j = 0; j < C::NM; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) st.o[j][r] *= move;
-        unit = now;
-        inv_unit = 1.f / now;
-        f = sv > 0.f ? 1.f : (sv < 0.f ? -1.f : sv);
-      }
+      for (int r = 0; r < 4; ++r) s[u][r] = exp2_approx(x[u][r]);
+      st.l[0] = fmaf(s[u][0] + s[u][2], back[u], st.l[0]);
+      st.l[1] = fmaf(s[u][1] + s[u][3], back[u], st.l[1]);
     }
   }
 
-  // O += f * (P V), P = s
-  __device__ __forceinline__ void values(float (&s)[4], float f, const char* vs) {
+  // O += P V, P = s * f
+  template <int N4, int N>
+  __device__ __forceinline__ void values(float (&s)[4], float f, const char* vs, const uint32_t (&vr)[N4][N]) {
     if constexpr (KIND == kSplitF32) {
       const int g = lane >> 2, t = lane & 3;
 #pragma unroll 4
@@ -865,7 +927,7 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
         }
       }
     } else {
-      if constexpr (C::k8 && kDirect) {
+      if constexpr (C::k8) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[r] *= f;
       }
@@ -909,7 +971,7 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
 #pragma unroll
           for (int x = 0; x < NP; ++x) split_mma<kPBf16>(d, m, b[x][0], b[x][1]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) st.o[j][r] = fmaf(f, d[r], st.o[j][r]);
+          for (int r = 0; r < 4; ++r) st.o[j][r] += d[r];
         }
       }
     }
@@ -919,10 +981,10 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
   // are one run of bytes each).
   __device__ __forceinline__ void ahead(const SplitParams& p, int j) const {
     if constexpr (C::k8 && kSplitAhead > S) {
-      if (lane < 2) {
-        const SplitPlace a = place(j);
+      if (lane < 2 * SUB) {
+        const SplitPlace a = place(j * SUB + (lane >> 1));
         if (a.mask & 0xffffu)
-          bulk_prefetch_l2(static_cast<const char*>(lane ? p.vc : p.kc) + a.page + (long long)a.off * E, 16 * E);
+          bulk_prefetch_l2(static_cast<const char*>(lane & 1 ? p.vc : p.kc) + a.page + (long long)a.off * E, 16 * E);
       }
     }
   }
@@ -930,32 +992,42 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
   // Tile j: true when its item ends.
   __device__ __forceinline__ bool step(const SplitParams& p, int j, int n) {
     if (j + kSplitAhead < n) ahead(p, j + kSplitAhead);
-    const uint32_t mask = place(j).mask;
-    const float2 sc = *reinterpret_cast<const float2*>(sm + R::kScaleAt + (j & (kSplitMeta - 1)) * 8);
+    uint32_t mask[SUB];
+    float4 sc[SUB];
+    float gv[SUB];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      mask[u] = place(j * SUB + u).mask;
+      if constexpr (C::k8)
+        sc[u] = *reinterpret_cast<const float4*>(sm + R::kScaleAt + ((j * SUB + u) & (kSplitMeta - 1)) * 16);
+    }
     char* at = slot(j);
-    float s[4], f;
-    split_wait<2 * S - 1>();
-    scores(s, at, mask);
+    float s[SUB][4];
+    if constexpr (R::kRing) split_wait<2 * S - 1>();
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) scores(s[u], at, mask[u], kr[u]);
     if (j + S < n) copy_k(p, j + S);
-    split_commit();
-    softmax(s, mask, sc.x, sc.y, f);
-    split_wait<2 * S - 1>();
+    if constexpr (R::kRing) split_commit();
+    softmax(s, mask, sc, gv);
+    if constexpr (R::kRing) split_wait<2 * S - 1>();
     if constexpr (C::kF32) __syncwarp();
-    values(s, f, at + R::kSide);
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) values(s[u], gv[u], at + R::kSide, vr[u]);
     if (j + S < n) copy_v(p, j + S);
-    split_commit();
-    return (mask >> 16) & 1;
+    if constexpr (R::kRing) split_commit();
+    return (mask[0] >> 16) & 1;
   }
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) st.l[x] += __shfl_xor_sync(0xffffffffu, st.l[x], o);
-    if constexpr (C::k8 && kDirect) {
+    if constexpr (C::k8) {
+      const float scale = exp2f(unit);
 #pragma unroll
       for (int x = 0; x < C::NM; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st.o[x][r] *= unit;
+        for (int r = 0; r < 4; ++r) st.o[x][r] *= scale;
     }
   }
 };
@@ -1024,7 +1096,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
     int sum = 0;
     for (int i = i0; i < i1; ++i) {
       prefix[i] = sum;  // (before the threads ahead are known)
-      sum += split_seq(p, i).nt;
+      sum += (split_seq(p, i).nt + split_sub<KIND, E>() - 1) / split_sub<KIND, E>();
     }
     const int incl = warp_scan_i(sum, lane);
     if (lane == 31) wsum[warp] = incl;
