@@ -45,7 +45,7 @@ struct AppendParams {
   long long total;   // packed: rows of key/value
   int n_new;         // tokens per sequence (dense), or the most of any (packed)
   int B, H, page;
-  int pages;  // pages a sequence touches at most
+  int pages;  // pages a sequence touches at most (packed: all of them)
   int* status;
 };
 
@@ -65,13 +65,12 @@ __device__ __forceinline__ int append_tokens(const AppendParams& p, int i, long 
   return (int)(z - a);
 }
 
-// The block of page pg of sequence i, or -1 (flagged).
-__device__ __forceinline__ int append_block(const AppendParams& p, int i, long long pg) {
+// Entry b of page pg of sequence i, or -1 (flagged).
+__device__ __forceinline__ int append_block(const AppendParams& p, int i, long long pg, int b) {
   if (pg >= p.pt_stride) {
     if (p.status) atomicOr(p.status, CA_STATUS_LENS);
     return -1;
   }
-  const int b = __ldg(p.page_table + i * p.pt_stride + pg);
   if (b < 0 || b >= p.num_blocks) {
     if (p.status) atomicOr(p.status, CA_STATUS_TABLE);
     return -1;
@@ -101,104 +100,226 @@ __device__ __forceinline__ float e4m3_scale(float top) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// VEC values from p (VEC16: one 16-byte load, else one value)
+// A 16-byte vector's values.
 template <typename T, int VEC>
-__device__ __forceinline__ void append_load(float (&x)[VEC], const T* p) {
-  if constexpr (VEC == 1) {
-    x[0] = to_f32(*p);
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void append_widen(float (&x)[VEC], const uint4& w) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if constexpr (sizeof(T) == 2) {
-        x[2 * c] = bf16_lo(u[c]);
-        x[2 * c + 1] = bf16_hi(u[c]);
-      } else {
-        x[c] = __uint_as_float(u[c]);
-      }
+  for (int c = 0; c < 4; ++c) {
+    if constexpr (sizeof(T) == 2) {
+      x[2 * c] = bf16_lo(u[c]);
+      x[2 * c + 1] = bf16_hi(u[c]);
+    } else {
+      x[c] = __uint_as_float(u[c]);
     }
   }
 }
+// VEC values from p (one 16-byte load, or one value)
+template <typename T, int VEC>
+__device__ __forceinline__ void append_load(float (&x)[VEC], const T* p) {
+  if constexpr (VEC == 1)
+    x[0] = to_f32(*p);
+  else
+    append_widen<T>(x, __ldg(reinterpret_cast<const uint4*>(p)));
+}
 
 constexpr int kAppendWarps = 4;
+constexpr int kAppendHeld = 8;  // vectors a lane keeps between the maximum and the codes
 
+// The largest magnitude of a vector's values and `top`, as bits (two bf16 at a
+// time: magnitudes order like whole numbers; infinities and NaN are the largest).
+template <typename T>
+__device__ __forceinline__ uint32_t append_top(const uint4& w, uint32_t top) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if constexpr (sizeof(T) == 2)
+      asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(u[c] & 0x7fff7fffu));
+    else
+      top = max(top, u[c] & 0x7fffffffu);
+  }
+  return top;
+}
+template <int VEC>
+__device__ __forceinline__ void append_codes(const float (&v)[VEC], uint8_t* dst) {
+  if constexpr (VEC == 8) {
+    const uint32_t w0 = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
+    const uint32_t w1 = e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+  } else if constexpr (VEC == 4) {
+    *reinterpret_cast<uint32_t*>(dst) = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
+  } else {
+    *dst = (uint8_t)e4m3x2(v[0], 0.f);
+  }
+}
+// The other codes of a block whose scale moved from `old` to `now`.
+__device__ __noinline__ void append_rescale(uint8_t* block, int bytes, int lo, int hi, float old, float now, int lane) {
+  const float ratio = __fdiv_rn(old, now);
+  uint32_t* w = reinterpret_cast<uint32_t*>(block);
+  for (int x = lane; x < bytes / 4; x += 32) {
+    if (4 * x >= lo && 4 * x < hi) continue;
+    const uint32_t c = w[x];
+    const float2 f0 = e4m3x2_to_f32(c), f1 = e4m3x2_to_f32(c >> 16);
+    w[x] = e4m3x2(f0.x * ratio, f0.y * ratio) | e4m3x2(f1.x * ratio, f1.y * ratio) << 16;
+  }
+}
+
+// A vector's values times inv, a power of two (bf16: two at a time, exact but
+// for results below bf16's normal range, whose codes are 0).
+template <typename T, int VEC>
+__device__ __forceinline__ void append_scaled(float (&v)[VEC], uint4 w, float inv) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162 by = __float2bfloat162_rn(inv);
+    __nv_bfloat162* u = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) u[c] = __hmul2(u[c], by);
+    append_widen<T>(v, w);
+  } else {
+    append_widen<T>(v, w);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) v[c] *= inv;
+  }
+}
+
+// Where packed sequence i's pages start among the launch's (their number grows
+// by at least what the sequence's tokens can touch).
+__device__ __forceinline__ long long append_start(const AppendParams& p, int i) {
+  return __ldg(p.cu + i) / p.page + 2LL * i;
+}
+// The last sequence that starts at or before page u (32 probes at a time).
+__device__ __forceinline__ int append_sequence(const AppendParams& p, long long u, int lane) {
+  int lo = 0, n = p.B;  // it is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lo + lane * step;
+    const bool before = lane * step < n && append_start(p, at) <= u;
+    const int k = max(0, __popc(__ballot_sync(0xffffffffu, before)) - 1);
+    n = min(step, n - k * step);
+    lo += k * step;
+  }
+  return lo;
+}
+
+// Grid: x = group of 4 (head, side) units of a page, y = sequence; packed: x =
+// all pages of all sequences, so short sequences beside long ones cost nothing.
+// The rows are loaded before the block id is known; a 16-token page of head_dim
+// 128 (bf16) stays in registers, so new tokens are read once.
 template <typename T, int E, bool VEC16>
 __global__ void __launch_bounds__(32 * kAppendWarps) append_8bit_kernel(const __grid_constant__ AppendParams p) {
   constexpr int VEC = VEC16 ? 16 / (int)sizeof(T) : 1;
-  constexpr int PER_ROW = E / VEC;
+  constexpr int PER_ROW = E / VEC;                            // vectors of a row
+  constexpr int LANES = PER_ROW < 32 ? PER_ROW : 32;          // lanes that share a row
+  constexpr int ROWS = 32 / LANES, STEPS = PER_ROW / LANES;   // rows a warp takes at a time, steps they take
   const int lane = threadIdx.x & 31;
-  // unit = ((sequence * pages + page) * H + head) * 2 + side
-  long long u = (long long)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
-  const int side = (int)(u & 1);
-  u >>= 1;
-  const int h = (int)(u % p.H);
-  u /= p.H;
-  const int pi = (int)(u % p.pages);
-  const long long i = u / p.pages;
-  if (i >= p.B) return;
-  const int before = __ldg(p.lens + i);
-  if (before < 0) return;
-  long long row;
-  const int n = append_tokens(p, (int)i, &row);
-  const long long pg = before / p.page + pi;
-  const long long p0 = pg * p.page;
-  const long long a = max((long long)before, p0), z = min((long long)before + n, p0 + p.page);
-  if (a >= z) return;
-  const int b = append_block(p, (int)i, pg);
-  if (b < 0) return;
-  const T* src = static_cast<const T*>(side ? p.value : p.key) + row + (a - before) * p.token_stride + (long long)h * E;
-  float* scale = (side ? p.vs : p.ks) + (long long)b * p.H + h;
-  uint8_t* dst = static_cast<uint8_t*>(side ? p.vc : p.kc) + ((long long)b * p.H + h) * p.page * E;
-  const int vecs = (int)(z - a) * PER_ROW;
-  const bool fresh = a == p0;
-  const float old = fresh ? 0.f : *scale;
+  const unsigned groups = (2u * p.H + kAppendWarps - 1) / kAppendWarps;
+  const int pi = (int)(blockIdx.x / groups);
+  const int unit = (int)(blockIdx.x - pi * groups) * kAppendWarps + (threadIdx.x >> 5);
+  if (unit >= 2 * p.H) return;
+  const int h = unit >> 1, side = unit & 1;
+  const int r0 = lane / LANES, c0 = (lane % LANES) * VEC;
+  const int first = p.cu ? append_sequence(p, pi, lane) : (int)blockIdx.y;
+  for (int i = first; i < p.B; i += p.cu ? p.B : (int)gridDim.y) {
+    const int before = __ldg(p.lens + i);
+    if (before < 0) continue;
+    long long row;
+    const int n = append_tokens(p, i, &row);
+    const int mine = p.cu ? (int)(pi - append_start(p, i)) : pi;  // of the pages the sequence touches
+    if (mine < 0) continue;
+    const int pg = before / p.page + mine;
+    const long long p0 = (long long)pg * p.page;
+    const long long a = max((long long)before, p0), z = min((long long)before + n, p0 + p.page);
+    if (a >= z) continue;
+    const int id = pg < p.pt_stride ? __ldg(p.page_table + i * p.pt_stride + pg) : -1;
+    const T* src = static_cast<const T*>(side ? p.value : p.key) + row + (a - before) * p.token_stride +
+                   (long long)h * E + r0 * p.token_stride + c0;
+    const long long down = ROWS * p.token_stride;
+    const int rows = (int)(z - a) - r0;  // of this lane: r0, r0 + ROWS, ...
+    uint4 held[kAppendHeld];
+    if constexpr (VEC16) {
+      const T* at = src;
+#pragma unroll
+      for (int k = 0; k < kAppendHeld; ++k, at += down) {
+        held[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (k * ROWS < rows) held[k] = __ldg(reinterpret_cast<const uint4*>(at));
+      }
+    }
+    const int b = append_block(p, i, pg, id);
+    if (b < 0) continue;
+    float* scale = (side ? p.vs : p.ks) + (long long)b * p.H + h;
+    uint8_t* block = static_cast<uint8_t*>(side ? p.vc : p.kc) + ((long long)b * p.H + h) * p.page * E;
+    const bool fresh = a == p0;
+    const float old = fresh ? 0.f : *scale;
 
-  float top = 0.f;
-#pragma unroll 4
-  for (int x = lane; x < vecs; x += 32) {
-    float v[VEC];
-    append_load<T, VEC>(v, src + (long long)(x / PER_ROW) * p.token_stride + (x % PER_ROW) * VEC);
+    // the largest magnitude; once more without what is not finite if there is any
+    uint32_t bits = 0u;
+    constexpr int kFirst = VEC16 ? kAppendHeld : 0;
+    if constexpr (VEC16) {
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) {
-      const float m = fabsf(v[c]);
-      if (m < INFINITY) top = fmaxf(top, m);
-    }
-  }
-  top = warp_max(top);
-  const float now = fmaxf(old, e4m3_scale(top));
-  // the block's other tokens, when the scale moved
-  if (!fresh && now != old) {
-    const float ratio = __fdiv_rn(old, now);
-    const int lo = (int)(a - p0) * E, hi = (int)(z - p0) * E;
-    uint32_t* w = reinterpret_cast<uint32_t*>(dst);
-    for (int x = lane; x < p.page * E / 4; x += 32) {
-      if (4 * x >= lo && 4 * x < hi) continue;
-      const uint32_t c = w[x];
-      const float2 f0 = e4m3x2_to_f32(c), f1 = e4m3x2_to_f32(c >> 16);
-      w[x] = e4m3x2(f0.x * ratio, f0.y * ratio) | e4m3x2(f1.x * ratio, f1.y * ratio) << 16;
-    }
-  }
-  // now is a power of two unless the caller's own scale was larger: then the
-  // quotient is rounded once before the code is
-  dst += (a - p0) * E;
-#pragma unroll 4
-  for (int x = lane; x < vecs; x += 32) {
-    float v[VEC];
-    append_load<T, VEC>(v, src + (long long)(x / PER_ROW) * p.token_stride + (x % PER_ROW) * VEC);
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) v[c] = __fdiv_rn(v[c], now);
-    if constexpr (VEC == 8) {
-      const uint32_t w0 = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
-      const uint32_t w1 = e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16;
-      *reinterpret_cast<uint2*>(dst + (long long)x * 8) = make_uint2(w0, w1);
-    } else if constexpr (VEC == 4) {
-      *reinterpret_cast<uint32_t*>(dst + (long long)x * 4) = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
+      for (int k = 0; k < kAppendHeld; ++k) bits = append_top<T>(held[k], bits);
+      const T* at = src + kFirst * down;
+      for (int k = kFirst; k * ROWS < rows; ++k, at += down)
+        bits = append_top<T>(__ldg(reinterpret_cast<const uint4*>(at)), bits);
+      if constexpr (sizeof(T) == 2) bits = max(bits & 0xffffu, bits >> 16) << 16;
     } else {
-      dst[x] = (uint8_t)e4m3x2(v[0], 0.f);
+      const T* at = src;
+      for (int k = 0; k * ROWS < rows; ++k, at += down)
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) bits = max(bits, __float_as_uint(to_f32(at[c * LANES])) & 0x7fffffffu);
     }
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    if (bits >= 0x7f800000u) {
+      bits = 0u;
+      const T* at = src;
+      for (int k = 0; k * ROWS < rows; ++k, at += down)
+        for (int c = 0; c < STEPS; ++c)
+          for (int e = 0; e < VEC; ++e) {
+            const uint32_t m = __float_as_uint(to_f32(at[c * LANES * VEC + e])) & 0x7fffffffu;
+            if (m < 0x7f800000u) bits = max(bits, m);
+          }
+      bits = __reduce_max_sync(0xffffffffu, bits);
+    }
+    const float now = fmaxf(old, e4m3_scale(__uint_as_float(bits)));
+    if (!fresh && now != old)
+      append_rescale(block, p.page * E, (int)(a - p0) * E, (int)(z - p0) * E, old, now, lane);
+    uint8_t* dst = block + ((int)(a - p0) + r0) * E + c0;
+    if ((__float_as_uint(now) & 0x7fffffu) == 0u) {
+      const float inv = 1.f / now;  // exact: now is a power of two
+      if constexpr (VEC16) {
+#pragma unroll
+        for (int k = 0; k < kAppendHeld; ++k)
+          if (k * ROWS < rows) {
+            float v[VEC];
+            append_scaled<T>(v, held[k], inv);
+            append_codes(v, dst + k * ROWS * E);
+          }
+      }
+      const T* at = src + kFirst * down;
+      for (int k = kFirst; k * ROWS < rows; ++k, at += down)
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+          float v[VEC];
+          if constexpr (VEC16) {
+            append_scaled<T>(v, __ldg(reinterpret_cast<const uint4*>(at + c * LANES * VEC)), inv);
+          } else {
+            append_load<T, VEC>(v, at + c * LANES * VEC);
+            v[0] *= inv;
+          }
+          append_codes(v, dst + k * ROWS * E + c * LANES * VEC);
+        }
+    } else {
+      // the caller's own scale was larger: the quotient is rounded once before the code is
+      const T* at = src;
+      for (int k = 0; k * ROWS < rows; ++k, at += down)
+        for (int c = 0; c < STEPS; ++c) {
+          float v[VEC];
+          append_load<T, VEC>(v, at + c * LANES * VEC);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = __fdiv_rn(v[e], now);
+          append_codes(v, dst + k * ROWS * E + c * LANES * VEC);
+        }
+    }
+    if (lane == 0 && now != old) *scale = now;
   }
-  if (lane == 0 && now != old) *scale = now;
 }
 
 // Float caches: one thread moves one element or 16-byte vector of a (sequence,
@@ -219,7 +340,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
   if (before < 0) return;
   const long long pos = (long long)before + j;
   const long long pg = pos / p.page;
-  const int b = append_block(p, (int)i, pg);
+  const int b = append_block(p, (int)i, pg, pg < p.pt_stride ? __ldg(p.page_table + i * p.pt_stride + pg) : -1);
   if (b < 0) return;
   const int off = (int)(pos - pg * p.page);
   const long long src = i * p.seq_stride + j * p.token_stride + (long long)h * E + v * VEC;

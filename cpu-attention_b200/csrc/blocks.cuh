@@ -2,7 +2,8 @@
 // plan that packs the blocks in use at the front of the pool.
 //
 // copy_blocks_kernel: pair (src, dst) of every tensor [num_blocks, ...]; a CTA
-// copies one block of one tensor. Bound by HBM: each byte read and written once.
+// copies one block of one tensor, or (blocks up to 1 KiB: scales) 64 pairs of it.
+// Bound by HBM: each byte read and written once.
 //
 // compact_plan_kernel (one CTA): with U the blocks that the page table's rows
 // use and n = |U|, the k-th smallest member of U that is >= n goes to the k-th
@@ -21,10 +22,13 @@ constexpr int kCopyThreads = 256;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxBlocks = 1 << 20;  // a 128 KiB bitmap
 
+constexpr int kCopySmall = 1024;  // bytes up to which a CTA takes kCopyGroup pairs of a tensor at a time
+constexpr int kCopyGroup = 64;
+
 struct CopyParams {
-  char* base[kCopyTensors];
+  char* base[kCopyTensors];       // those with large blocks first
   long long bytes[kCopyTensors];  // per block
-  int tensors;
+  int tensors, large;
   long long num_blocks;
   const long long* pairs;  // [n][2] (src, dst), or NULL: moves
   const int* moves;        // [n][2]
@@ -33,52 +37,93 @@ struct CopyParams {
   int* status;
 };
 
+// 8 words a thread in flight.
 template <typename W>
 __device__ __forceinline__ void copy_words(char* dst, const char* src, long long bytes) {
   const W* s = reinterpret_cast<const W*>(src);
   W* d = reinterpret_cast<W*>(dst);
   const long long n = bytes / (long long)sizeof(W);
   constexpr int U = 8;
-  long long x = threadIdx.x;
-  for (; x + (U - 1) * kCopyThreads < n; x += U * kCopyThreads) {
+  for (long long x0 = 0; x0 < n; x0 += U * kCopyThreads) {
+    const int left = (int)min((long long)U * kCopyThreads, n - x0);
     W r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = s[x + u * kCopyThreads];
+    for (int u = 0; u < U; ++u) {
+      const int x = threadIdx.x + u * kCopyThreads;
+      if (x < left) r[u] = s[x0 + x];
+    }
 #pragma unroll
-    for (int u = 0; u < U; ++u) d[x + u * kCopyThreads] = r[u];
+    for (int u = 0; u < U; ++u) {
+      const int x = threadIdx.x + u * kCopyThreads;
+      if (x < left) d[x0 + x] = r[u];
+    }
   }
-  for (; x < n; x += kCopyThreads) d[x] = s[x];
+}
+
+// (src, dst) of a pair; false when it is left out.
+__device__ __forceinline__ bool copy_pair(const CopyParams& p, long long pair, long long* src, long long* dst) {
+  if (p.pairs) {
+    *src = __ldg(p.pairs + 2 * pair);
+    *dst = __ldg(p.pairs + 2 * pair + 1);
+    if (*src < 0 || *dst < 0) return false;  // padding
+    if (*src >= p.num_blocks || *dst >= p.num_blocks) {
+      if (p.status) atomicOr(p.status, CA_STATUS_SLOT);
+      return false;
+    }
+  } else {
+    *src = __ldg(p.moves + 2 * pair);
+    *dst = __ldg(p.moves + 2 * pair + 1);
+  }
+  return *src != *dst;
+}
+
+template <typename W>
+__device__ __forceinline__ void copy_group(const CopyParams& p, char* base, int bytes, long long first, int pairs) {
+  const int per = bytes / (int)sizeof(W);
+  for (int x = threadIdx.x; x < pairs * per; x += kCopyThreads) {
+    const int k = x / per, w = x - k * per;
+    long long src, dst;
+    if (!copy_pair(p, first + k, &src, &dst)) continue;
+    reinterpret_cast<W*>(base + dst * bytes)[w] = reinterpret_cast<const W*>(base + src * bytes)[w];
+  }
 }
 
 __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const __grid_constant__ CopyParams p) {
   const long long n = p.pairs ? p.n : __ldg(p.count);
-  for (long long u = blockIdx.x; u < n * p.tensors; u += gridDim.x) {
-    const long long pair = u / p.tensors;
-    const int t = (int)(u - pair * p.tensors);
-    long long src, dst;
-    if (p.pairs) {
-      src = __ldg(p.pairs + 2 * pair);
-      dst = __ldg(p.pairs + 2 * pair + 1);
-      if (src < 0 || dst < 0) continue;  // padding
-      if (src >= p.num_blocks || dst >= p.num_blocks) {
-        if (p.status && threadIdx.x == 0) atomicOr(p.status, CA_STATUS_SLOT);
-        continue;
-      }
+  const int small = p.tensors - p.large;
+  const long long groups = (n + kCopyGroup - 1) / kCopyGroup;
+  // units: a pair of a tensor with large blocks, then a group of pairs of one with small blocks
+  for (long long u = blockIdx.x; u < n * p.large + groups * small; u += gridDim.x) {
+    if (u < n * p.large) {
+      const unsigned long long pair = u <= 0xffffffffLL ? (unsigned)u / (unsigned)p.large : u / p.large;
+      const int t = (int)(u - pair * p.large);
+      long long src, dst;
+      if (!copy_pair(p, pair, &src, &dst)) continue;
+      const long long bytes = p.bytes[t];
+      const char* s = p.base[t] + src * bytes;
+      char* d = p.base[t] + dst * bytes;
+      const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
+      if ((at & 15) == 0)
+        copy_words<uint4>(d, s, bytes);
+      else if ((at & 3) == 0)
+        copy_words<uint32_t>(d, s, bytes);
+      else
+        copy_words<uint8_t>(d, s, bytes);
     } else {
-      src = __ldg(p.moves + 2 * pair);
-      dst = __ldg(p.moves + 2 * pair + 1);
+      const long long v = u - n * p.large;
+      const long long group = v / small;
+      const int t = p.large + (int)(v - group * small);
+      const int bytes = (int)p.bytes[t];
+      const long long first = group * kCopyGroup;
+      const int pairs = (int)min((long long)kCopyGroup, n - first);
+      const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
+      if ((at & 15) == 0)
+        copy_group<uint4>(p, p.base[t], bytes, first, pairs);
+      else if ((at & 3) == 0)
+        copy_group<uint32_t>(p, p.base[t], bytes, first, pairs);
+      else
+        copy_group<uint8_t>(p, p.base[t], bytes, first, pairs);
     }
-    if (src == dst) continue;
-    const long long bytes = p.bytes[t];
-    const char* s = p.base[t] + src * bytes;
-    char* d = p.base[t] + dst * bytes;
-    const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
-    if ((at & 15) == 0)
-      copy_words<uint4>(d, s, bytes);
-    else if ((at & 3) == 0)
-      copy_words<uint32_t>(d, s, bytes);
-    else
-      copy_words<uint8_t>(d, s, bytes);
   }
 }
 

@@ -17,11 +17,11 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) %
 template <typename T, int E>
 int launch_append(const ca::AppendParams& prm, bool eight, bool vec16, cudaStream_t stream) {
   if (eight) {
-    const long long units = 2LL * prm.B * prm.pages * prm.H;
-    const long long ctas = (units + ca::kAppendWarps - 1) / ca::kAppendWarps;
+    const long long ctas = (long long)prm.pages * ((2 * prm.H + ca::kAppendWarps - 1) / ca::kAppendWarps);
     if (ctas > 0x7fffffffLL) return CA_EUNSUPPORTED;
     auto kern = vec16 ? ca::append_8bit_kernel<T, E, true> : ca::append_8bit_kernel<T, E, false>;
-    kern<<<(unsigned)ctas, 32 * ca::kAppendWarps, 0, stream>>>(prm);
+    const dim3 grid((unsigned)ctas, prm.cu ? 1u : (unsigned)std::min(prm.B, 65535));
+    kern<<<grid, 32 * ca::kAppendWarps, 0, stream>>>(prm);
   } else {
     const long long per_row = vec16 ? E / (16 / (int)sizeof(T)) : E;
     const long long ctas = ((long long)prm.B * prm.n_new * prm.H * per_row + 255) / 256;
@@ -79,7 +79,9 @@ int append_plan(ca::AppendParams* prm, const void* key, const void* value, int64
   prm->B = (int)batch;
   prm->H = (int)heads;
   prm->page = (int)page;
-  prm->pages = (int)((n_new + page - 2) / page + 1);
+  const int64_t pages = cu ? total / page + 2 * batch : (n_new + page - 2) / page + 1;
+  if (pages > 0x7fffffffLL) return CA_EUNSUPPORTED;
+  prm->pages = (int)pages;
   prm->status = status;
   return CA_OK;
 }
@@ -93,9 +95,14 @@ bool sizes_ok(int64_t batch, int64_t heads, int64_t num_blocks, int64_t table_wi
 int copy_params(ca::CopyParams* prm, void* const* base, const int64_t* bytes, int64_t first, int64_t tensors,
                 int64_t num_blocks, int32_t* status) {
   prm->tensors = (int)std::min<int64_t>(ca::kCopyTensors, tensors - first);
-  for (int t = 0; t < prm->tensors; ++t) {
-    prm->base[t] = static_cast<char*>(base[first + t]);
-    prm->bytes[t] = bytes[first + t];
+  int at = 0;
+  for (int small = 0; small < 2; ++small) {
+    for (int t = 0; t < prm->tensors; ++t)
+      if ((bytes[first + t] <= ca::kCopySmall) == (small != 0)) {
+        prm->base[at] = static_cast<char*>(base[first + t]);
+        prm->bytes[at++] = bytes[first + t];
+      }
+    if (!small) prm->large = at;
   }
   prm->num_blocks = num_blocks;
   prm->status = status;
