@@ -155,6 +155,7 @@ __device__ __forceinline__ int tc_tiles(int r0, int Lq, int Lk, bool causal) {
 // `skip` tiles later, those from its first row's window on.
 struct TcTiles {
   int ns, skip;
+  int late;  // tiles [ns, ns + late) lie before every window of query tile B, which leaves them out
   __device__ __forceinline__ int real(int j) const { return j < ns ? j : j + skip; }
 };
 
@@ -187,12 +188,11 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
   const int tb = a.cu_q ? 0 : b;             // TMA batch coordinate
   const int tq = (int)sq.tq0, tk = (int)sq.tk0;  // TMA token offsets (varlen)
   int nt0 = tc_tiles(q0, Lq, Lk, CAUSAL), nt1 = tc_tiles(q0 + C::BM, Lq, Lk, CAUSAL);
-  TcTiles tiles{0, 0};
+  TcTiles tiles{0, 0, 0};
   if constexpr (WIN) {
-    // tiles are numbered without those that no row of the CTA sees (tile B
-    // starts with A's: the rows of B mask what lies before their window). A
-    // row's window ends at or after its start, so a query tile that sees
-    // anything has tiles past the skipped ones.
+    // tiles are numbered without those that no row of the CTA sees. A row's
+    // window ends at or after its start, so a query tile that sees anything has
+    // tiles past the skipped ones.
     auto count = [&](int r0) {
       if (r0 >= Lq) return 0;
       return (max(0, flash_window(a, min(r0 + C::BM, Lq) - 1, Lq, Lk).hi + 1) + C::BN - 1) / C::BN;
@@ -203,7 +203,19 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
     tiles.skip = max(0, (q0 < Lq ? flash_window(a, q0, Lq, Lk).lo : 0) / C::BN - tiles.ns);
     nt0 = max(0, nt0 - tiles.skip);
     nt1 = max(0, nt1 - tiles.skip);
+    if (nt1 > 0)
+      tiles.late = max(0, flash_window(a, q0 + C::BM, Lq, Lk).lo / C::BN - tiles.ns - tiles.skip);
   }
+  // whether query tile x reads tile j, and how many it has read before it
+  auto uses = [&](int x, int j) {
+    if constexpr (WIN)
+      if (x && j >= tiles.ns && j < tiles.ns + tiles.late) return false;
+    return j < (x ? nt1 : nt0);
+  };
+  auto seq = [&](int x, int j) {
+    if constexpr (WIN) return x && j >= tiles.ns ? j - tiles.late : j;
+    return j;
+  };
   const int nt = max(nt0, nt1);
 
   if (threadIdx.x == 0) {
@@ -305,7 +317,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       // O_x += P_x(j) V_j; the last user of V_j releases its slot
       auto issue_pv = [&](int x, int j) -> bool {
         const int vs = j % C::VST;
-        if (!tc_wait(&bars->p[x], j & 1, abort, a.status)) return false;
+        if (!tc_wait(&bars->p[x], seq(x, j) & 1, abort, a.status)) return false;
         if (!tc_wait(&bars->vf[vs], (j / C::VST) & 1, abort, a.status)) return false;
         tc::fence_after_sync();
         const uint32_t vaddr = smem_u32(sV + vs * C::TILE_BYTES);
@@ -313,18 +325,20 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
         for (int kk = 0; kk < C::BN / 16; ++kk)
           tc::mma_ts(tmem + C::T_O(x), tmem + C::T_S(x) + kk * 8,
                      tc::smem_desc(vaddr + kk * 16 * C::SWB, C::CH_BYTES, 8 * C::SWB, C::SWZ), idO,
-                     (j > 0 || kk > 0) ? 1u : 0u);
+                     (seq(x, j) > 0 || kk > 0) ? 1u : 0u);
         tc::commit(&bars->pv[x]);
         return true;
       };
-      if (ok && nt0 > 0) ok = issue_s(0, 0);
-      if (ok && nt1 > 0) ok = issue_s(1, 0);
+      if (ok && uses(0, 0)) ok = issue_s(0, 0);
+      if (ok && uses(1, 0)) ok = issue_s(1, 0);
       for (int j = 0; ok && j < nt; ++j) {
         for (int x = 0; ok && x < 2; ++x) {
-          if (j >= (x ? nt1 : nt0)) continue;
-          ok = issue_pv(x, j);
+          if (uses(x, j))
+            ok = issue_pv(x, j);
+          else if (!WIN)
+            continue;
           // S_x(j+1) overwrites S_x/P_x: issued after PV_x(j), tcgen05.mma runs in order
-          if (ok && j + 1 < (x ? nt1 : nt0)) ok = issue_s(x, j + 1);
+          if (ok && uses(x, j + 1)) ok = issue_s(x, j + 1);
         }
       }
       // every MMA this thread issued has retired before TMEM is released
@@ -347,14 +361,17 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       lim = w.hi;
       low = w.lo;
     }
-    const int ntr = (x ? nt1 : nt0);
+    const int nend = (x ? nt1 : nt0);
+    const int ntr = nend > 0 ? seq(x, nend - 1) + 1 : 0;  // tiles this query tile reads
     // masked scores get a value that scale * value maps to -inf
     const float sent = a.c >= 0.f ? -INFINITY : INFINITY;
     const uint64_t c2v = f32x2(a.c, a.c);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < ntr; ++j) {
-      if (!__all_sync(0xffffffffu, tc_wait(&bars->s[x], j & 1, abort, a.status))) {
+    for (int n = 0; n < ntr; ++n) {
+      const int j = WIN && x && n >= tiles.ns ? n + tiles.late : n;
+      const int prev = WIN && x && n - 1 >= tiles.ns ? n - 1 + tiles.late : n - 1;  // the tile read before
+      if (!__all_sync(0xffffffffu, tc_wait(&bars->s[x], n & 1, abort, a.status))) {
         ok = false;
         break;
       }
@@ -364,8 +381,8 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       // of V_{j-1}, those ring slots are free again. Arriving here instead of
       // committing from the MMA thread keeps the MMA issuer on MMAs.
       if (grp == 0 && lane == 0) {
-        if (x == (j < nt1 ? 1 : 0)) mbar_arrive(&bars->ke[j % C::KST]);
-        if (j >= 1 && x == (j - 1 < nt1 ? 1 : 0)) mbar_arrive(&bars->ve[(j - 1) % C::VST]);
+        if (x == (uses(1, j) ? 1 : 0)) mbar_arrive(&bars->ke[j % C::KST]);
+        if (n >= 1 && x == (uses(1, prev) ? 1 : 0)) mbar_arrive(&bars->ve[prev % C::VST]);
       }
       // the whole S row in registers: one TMEM round trip per tile
       uint32_t sr[C::BN];
@@ -376,17 +393,21 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       bool full = (k0 + C::BN - 1) <= lim;
       // windowed: one bit per key of the tile that this row sees
       uint32_t seen[WIN ? C::BN / 32 : 1];
+      uint32_t none = 0u;  // bit w: no row of the warp sees anything of columns [32w, 32w + 32)
       if constexpr (WIN) {
         full = full && (k0 >= low || k0 + C::BN <= a.sinks);
-        if (!full) {
+        if (!__all_sync(0xffffffffu, full)) {
 #pragma unroll
           for (int w = 0; w < C::BN / 32; ++w) {
             const int at = k0 + 32 * w;
             seen[w] = bit_range(low - at, lim + 1 - at) | bit_range(0, min(a.sinks, lim + 1) - at);
-          }
+            if (!__all_sync(0xffffffffu, seen[w] == 0xffffffffu)) {
 #pragma unroll
-          for (int i = 0; i < C::BN; ++i)
-            if (!((seen[i / 32] >> (i % 32)) & 1u)) sr[i] = __float_as_uint(sent);
+              for (int i = 0; i < 32; ++i)
+                if (!((seen[w] >> i) & 1u)) sr[32 * w + i] = __float_as_uint(sent);
+              if (!__any_sync(0xffffffffu, seen[w] != 0u)) none |= 1u << w;
+            }
+          }
         } else {
 #pragma unroll
           for (int w = 0; w < C::BN / 32; ++w) seen[w] = 0xffffffffu;
@@ -433,6 +454,14 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
           // packed pair i of this chunk goes to sr[32ch + i]: it was read (as
           // element 2i >= i of the chunk) before it is overwritten
           uint32_t* pk = sr + ch * 32;
+          if constexpr (WIN) {
+            if (none >> ch & 1u) {  // (uniform) the first keys' tile is mostly this
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0u;
+              tc::tmem_st16(tS + ch * 16, *reinterpret_cast<const uint32_t(*)[16]>(pk));
+              continue;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int e0 = ch * 32 + 2 * i;
@@ -451,7 +480,9 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
           tc::tmem_st16(tS + ch * 16, *reinterpret_cast<const uint32_t(*)[16]>(pk));
         }
       };
-      if (__all_sync(0xffffffffu, full))
+      // (windowed: a masked score is -inf by now, and its exponential 0 but for a
+      // scale of 0)
+      if (__all_sync(0xffffffffu, full) || (WIN && a.c != 0.f))
         exp_row(std::false_type{});
       else
         exp_row(std::true_type{});
@@ -459,8 +490,8 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       l = fmaf(l, alpha, sum);
       m = mn;
       // rescale O (holding tiles < j) when the max moved
-      if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        if (!__all_sync(0xffffffffu, tc_wait(&bars->pv[x], (j - 1) & 1, abort, a.status))) {
+      if (n >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (!__all_sync(0xffffffffu, tc_wait(&bars->pv[x], (n - 1) & 1, abort, a.status))) {
           ok = false;
           break;
         }
