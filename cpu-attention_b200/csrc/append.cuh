@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_8bit_kernel(const __
   constexpr int PER_ROW = E / VEC;                            // vectors of a row
   constexpr int LANES = PER_ROW < 32 ? PER_ROW : 32;          // lanes that share a row
   constexpr int ROWS = 32 / LANES, STEPS = PER_ROW / LANES;   // rows a warp takes at a time, steps they take
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (a decode waits before it reads the cache)
   const int lane = threadIdx.x & 31;
   const unsigned groups = (2u * p.H + kAppendWarps - 1) / kAppendWarps;
   const int pi = (int)(blockIdx.x / groups);
@@ -328,6 +329,7 @@ template <typename T, int E, bool VEC16>
 __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant__ AppendParams p) {
   constexpr int VEC = VEC16 ? 16 / (int)sizeof(T) : 1;
   constexpr int PER_ROW = E / VEC;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (a decode waits before it reads the cache)
   const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const int v = (int)(idx % PER_ROW);
   long long r = idx / PER_ROW;

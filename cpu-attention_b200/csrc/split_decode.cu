@@ -7,7 +7,7 @@ namespace ca {
 namespace {
 
 template <int KIND, typename QT, int E>
-cudaError_t launch(SplitParams prm, int ctas, int device, cudaStream_t stream) {
+cudaError_t launch(SplitParams prm, int ctas, bool after_append, int device, cudaStream_t stream) {
   const int smem = split_smem_fixed<KIND, E>() + 4 * (prm.B + 1);
   auto kern = split_decode_kernel<KIND, QT, E>;
   static unsigned char configured[64] = {};
@@ -18,28 +18,33 @@ cudaError_t launch(SplitParams prm, int ctas, int device, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     configured[device] = 1;  // (a race sets the same value twice)
   }
-  kern<<<ctas, 32 * kSplitWarps, smem, stream>>>(prm);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  // the join of items cut by a CTA boundary starts as the decode drains
+  // Each launch may start while the one before drains: the decode behind an
+  // append of this call (up to its first look at the cache), the join of items
+  // cut by a CTA boundary behind the decode.
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(32 * kSplitMergeShares * (E / 16));
+  cfg.blockDim = dim3(32 * kSplitWarps);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
+  cfg.attrs = &early;
+  cfg.numAttrs = after_append ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
+  if (e != cudaSuccess) return e;
+  cfg.blockDim = dim3(32 * kSplitMergeShares * (E / 16));
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, split_merge_kernel<KIND, QT, E>, prm);
 }
 
 template <int KIND, typename QT>
-cudaError_t by_dim(const SplitParams& prm, int head_dim, int ctas, int device, cudaStream_t s) {
+cudaError_t by_dim(const SplitParams& prm, int head_dim, int ctas, bool after, int device, cudaStream_t s) {
   switch (head_dim) {
-    case 32: return launch<KIND, QT, 32>(prm, ctas, device, s);
-    case 64: return launch<KIND, QT, 64>(prm, ctas, device, s);
-    default: return launch<KIND, QT, 128>(prm, ctas, device, s);
+    case 32: return launch<KIND, QT, 32>(prm, ctas, after, device, s);
+    case 64: return launch<KIND, QT, 64>(prm, ctas, after, device, s);
+    default: return launch<KIND, QT, 128>(prm, ctas, after, device, s);
   }
 }
 
@@ -87,14 +92,15 @@ cudaError_t split_launch(const SplitCall& c, int sms, int device, cudaStream_t s
     prm.partial = static_cast<float*>(c.workspace);
     prm.meta = reinterpret_cast<int*>(prm.partial + (size_t)ctas * 2 * piece_bytes(c.head_dim) / 4);
     prm.status = c.status;
+    const bool after = c.n_new > 0 && b0 == 0;  // the launch before this one is the append
     cudaError_t e;
     if (c.cache_dtype == CA_DTYPE_E4M3)
-      e = c.q_dtype == CA_DTYPE_BF16 ? by_dim<kSplitE4m3, __nv_bfloat16>(prm, c.head_dim, ctas, device, stream)
-                                     : by_dim<kSplitE4m3, float>(prm, c.head_dim, ctas, device, stream);
+      e = c.q_dtype == CA_DTYPE_BF16 ? by_dim<kSplitE4m3, __nv_bfloat16>(prm, c.head_dim, ctas, after, device, stream)
+                                     : by_dim<kSplitE4m3, float>(prm, c.head_dim, ctas, after, device, stream);
     else if (c.cache_dtype == CA_DTYPE_BF16)
-      e = by_dim<kSplitBf16, __nv_bfloat16>(prm, c.head_dim, ctas, device, stream);
+      e = by_dim<kSplitBf16, __nv_bfloat16>(prm, c.head_dim, ctas, after, device, stream);
     else
-      e = by_dim<kSplitF32, float>(prm, c.head_dim, ctas, device, stream);
+      e = by_dim<kSplitF32, float>(prm, c.head_dim, ctas, after, device, stream);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

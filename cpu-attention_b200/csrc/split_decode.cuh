@@ -65,7 +65,7 @@ constexpr int kSplitAhead = 2;        // tiles ahead whose lines are brought to 
 // may pass by kSlack before it moves (a vote per tile, no reduction): up to 2^14
 // for f16, whose smallest step is then 2^-30 of the reference's weight.
 constexpr float kUp = 6.f, kSlack = 8.f;
-constexpr int kSplitMergeShares = 4;
+constexpr int kSplitMergeShares = 2;
 
 struct SplitParams {
   const void* q;
@@ -507,13 +507,13 @@ struct SplitWalk {
       // the next places, in three steps so that no load is waited for (the
       // ring runs S <= 8 tiles ahead)
       const int phase = j & (kBatch - 1);
-      if (j - phase + kBatch < n) {
+      if (__builtin_expect(j - phase + kBatch < n, 0)) {
         if (phase == 0) place_begin(p, prefix);
         if (phase == kBatch / 4) place_scales(p);
         if (phase == kBatch / 2) place_store(p, j + kBatch / 2);
       }
       const bool ends = w.step(p, j, n);
-      if (ends || j == n - 1) {
+      if (__builtin_expect(ends || j == n - 1, 0)) {
         w.finish();
         done(i, ih, starts, ends);
         if (j < n - 1) {
@@ -837,7 +837,7 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
       e[u] = 0.f;
       back[u] = gv[u] = 1.f;
       if constexpr (C::k8)
-        if (sc[u].y > unit) follow(sc[u].y);  // (uniform)
+        if (__builtin_expect(sc[u].y > unit, 0)) follow(sc[u].y);  // (uniform)
     }
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
@@ -861,7 +861,7 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
     }
     // a weight past 2^(kUp + kSlack) (or one that is no number, as all are
     // before a column has a reference) moves the references
-    if (__any_sync(0xffffffffu, !fits)) {
+    if (__builtin_expect(__any_sync(0xffffffffu, !fits), 0)) {
       float mt[2] = {-INFINITY, -INFINITY}, alpha[2];
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
@@ -1116,14 +1116,21 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
   const long long w1 = min(total, w0 + chunk);
 
   // ---- this warp's tiles
-  if (w0 < w1) {
-    SplitSpot a = split_spot(prefix, p.B, p.IH, w0);
-    const int n = (int)(split_spot(prefix, p.B, p.IH, w1).tile - a.tile);
-    if (n > 0) {
-      while (prefix[a.i + 1] == prefix[a.i]) {  // sequences that see nothing have no tiles
-        ++a.i;
-        a.ih = a.v = 0;
-      }
+  // (lane 1 looks up the end while the others look up the start)
+  SplitSpot a = split_spot(prefix, p.B, p.IH, lane == 1 ? w1 : w0);
+  const int n = w0 < w1 ? (int)(__shfl_sync(0xffffffffu, a.tile, 1) - __shfl_sync(0xffffffffu, a.tile, 0)) : 0;
+  a.i = __shfl_sync(0xffffffffu, a.i, 0);
+  a.ih = __shfl_sync(0xffffffffu, a.ih, 0);
+  a.v = __shfl_sync(0xffffffffu, a.v, 0);
+  if (n > 0)
+    while (prefix[a.i + 1] == prefix[a.i]) {  // sequences that see nothing have no tiles
+      ++a.i;
+      a.ih = a.v = 0;
+    }
+  // What an append just before this launch writes is read from here on. (Every
+  // warp waits: what follows in the stream waits for this launch only.)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (n > 0) {
       SplitWarp<KIND, QT, E> w;
       w.sm = split_smem + warp * kWarpBytes;
       w.lane = lane;
@@ -1135,7 +1142,6 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
           if (lane == 0) info[warp * 2 + (starts ? 1 : 0)] = SplitPiece{i, ih, ends ? 1 : 0, 1};
         }
       });
-    }
   }
   // ---- sequences that see nothing: zeros
   for (int i = blockIdx.x; i < p.B; i += gridDim.x)
