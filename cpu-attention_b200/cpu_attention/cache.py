@@ -81,6 +81,27 @@ def check_eight_bit(k_cache, v_cache, k_descale, v_descale):
                              "contiguous")
 
 
+def check_packed_caches(k_cache, v_cache):
+    """Raise unless the kernels can read the caches' 16-byte vectors."""
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("cpu_attention: the paged caches must be contiguous")
+    if any(t.numel() and t.data_ptr() % 16 for t in (k_cache, v_cache)):
+        raise ValueError("cpu_attention: the paged caches must start at a multiple of 16 bytes")
+
+
+def packed_rows(*ts):
+    """Copies of the tensors with the strides of a fresh tensor (a size of 1 may
+    have any stride in one that is contiguous), all or none."""
+    def plain(t):
+        want, n = [], 1
+        for size in reversed(t.shape):
+            want.append(n)
+            n *= max(size, 1)
+        return t.stride() == tuple(reversed(want))
+    return ts if all(map(plain, ts)) else tuple(t.clone(memory_format=torch.contiguous_format).view(-1).view(t.shape)
+                                                for t in ts)
+
+
 def append_quantized(key, value, k_cache, v_cache, k_descale, v_descale, cache_seqlens, page_table,
                      cu_seqlens_new=None, max_seqlen_new=None) -> None:
     """Appends tokens to paged caches held in 8 bits.
@@ -134,8 +155,7 @@ def _explain_append(key, value, k_cache, v_cache, k_scale, v_scale, lens, table,
         raise ValueError("cpu_attention: key/value heads or head_dim do not match the cache")
     if key.dtype not in K.DTYPES or value.dtype != key.dtype:
         raise ValueError("cpu_attention: key/value must share a dtype (fp32 or bf16)")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError("cpu_attention: the paged caches must be contiguous")
+    check_packed_caches(k_cache, v_cache)
     if hd not in K.HEAD_DIMS or page % 16 or page < 1 or heads < 1:
         raise ValueError("cpu_attention: head_dim must be 32/64/128 and the page a multiple of 16")
     if lens.dtype != torch.int32 or lens.dim() != 1:
@@ -164,7 +184,7 @@ def _explain_append(key, value, k_cache, v_cache, k_scale, v_scale, lens, table,
     if dev.type != "cuda" or any(t.device != dev for t in (key, value, v_cache, k_scale, v_scale)):
         raise ValueError("cpu_attention: key/value, the caches and their scales must be CUDA tensors on one device "
                          f"(the cache is on {dev})")
-    key, value = key.contiguous(), value.contiguous()
+    key, value = packed_rows(key, value)
     lens, table, cu = (x if x is None else x.contiguous().to(dev) for x in (lens, table, cu))
     return key, value, k_cache, v_cache, k_scale, v_scale, lens, table, cu
 

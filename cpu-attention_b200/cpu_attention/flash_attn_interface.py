@@ -21,7 +21,7 @@ import torch
 
 from . import _kernel as K
 from . import _native
-from .cache import check_eight_bit, reshape_and_cache
+from .cache import check_eight_bit, check_packed_caches, packed_rows, reshape_and_cache
 
 # flash_attn_with_kvcache options no kernel here implements; setting one raises
 _NOT_SUPPORTED = ("cpu_attention: qv, rotary, cache_leftpad, varlen, descale of float caches, sliding windows without "
@@ -128,9 +128,9 @@ def flash_attn_with_kvcache(
     # the option table -- an engine calls this once per layer and token)
     if not (qv is None and rotary_cos is None and rotary_sin is None and cache_leftpad is None
             and cu_seqlens_q is None and cu_seqlens_k_new is None and max_seqlen_q is None
-            and rotary_seqlens is None and q_descale is None and k_descale is None and v_descale is None
-            and alibi_slopes is None and sink_tokens is None and not attention_chunk and not softcap
-            and window_size == (-1, -1)) \
+            and rotary_seqlens is None and q_descale is None and alibi_slopes is None and not attention_chunk
+            and not softcap and (window_size == (-1, -1) or sink_tokens is not None)
+            and (k_descale is None and v_descale is None or k_cache.dtype == K.EIGHT_BIT)) \
             and _options_set(dict(qv=qv, rotary_cos=rotary_cos, rotary_sin=rotary_sin, cache_leftpad=cache_leftpad,
                                   cu_seqlens_q=cu_seqlens_q, cu_seqlens_k_new=cu_seqlens_k_new,
                                   max_seqlen_q=max_seqlen_q, rotary_seqlens=rotary_seqlens, q_descale=q_descale,
@@ -204,7 +204,8 @@ def _window(window_size, sink_tokens):
     if left < -1 or right < -1 or sinks < 0:
         raise ValueError("cpu_attention: window_size must be (left, right) of -1 or more and sink_tokens 0 or more "
                          f"(got {tuple(window_size)}, {sink_tokens})")
-    return left, right, min(sinks, 1 << 30)
+    most = 0x7fffff00  # past every length
+    return min(left, most), min(right, most), min(sinks, most)
 
 
 def _explain_split(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table):
@@ -227,8 +228,7 @@ def _explain_split(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table):
     kv_heads = k_cache.shape[1]
     if k_cache.shape[3] != hd or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("cpu_attention: q and the caches disagree on heads or head_dim")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError("cpu_attention: the paged caches must be contiguous")
+    check_packed_caches(k_cache, v_cache)
     if q.dtype not in K.DTYPES or (not eight and (k_cache.dtype != q.dtype or v_cache.dtype != q.dtype)):
         raise ValueError("cpu_attention: q and the caches must share a dtype (fp32 or bf16)")
     if hd not in K.HEAD_DIMS or k_cache.shape[2] % 16 or k_cache.shape[2] < 1:
@@ -252,8 +252,8 @@ def _explain_split(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table):
         raise ValueError("cpu_attention: q, the caches and k/v must be CUDA tensors on one device "
                          f"(q is on {dev})")
     if k is not None:
-        k, v = k.contiguous(), v.contiguous()
-    q = q.contiguous()
+        k, v = packed_rows(k, v)
+    (q,) = packed_rows(q)
     return (q, k_cache, v_cache, k, v, k_scale, v_scale, _to(lens.contiguous(), dev), _to(table.contiguous(), dev))
 
 

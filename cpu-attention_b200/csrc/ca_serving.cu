@@ -54,9 +54,10 @@ int append_plan(ca::AppendParams* prm, const void* key, const void* value, int64
                 int64_t num_blocks, const int32_t* lens, const int32_t* page_table, int64_t table_width,
                 int64_t batch, int64_t heads, int64_t head_dim, int64_t page, int dtype, int32_t* status,
                 bool* vec16) {
-  if (!key || !value || !kc || !vc || !lens || !page_table) return CA_ENULL;
+  // (an empty pool or table has no address, and is not read)
+  if (!key || !value || !lens || (num_blocks && (!kc || !vc)) || (table_width && !page_table)) return CA_ENULL;
   const size_t es = elem_size(dtype);
-  if (token_stride < heads * head_dim && (n_new > 1 || cu)) return CA_ELAYOUT;
+  if (token_stride < heads * head_dim && (cu ? total > 1 : n_new > 1)) return CA_ELAYOUT;
   if (!cu && seq_stride < (n_new > 1 ? n_new * token_stride : heads * head_dim) && batch > 1) return CA_ELAYOUT;
   if (!aligned(key, es) || !aligned(value, es) || !aligned(kc, 16) || !aligned(vc, 16)) return CA_ELAYOUT;
   *vec16 = aligned(key, 16) && aligned(value, 16) && (cu || (seq_stride * es) % 16 == 0) &&
@@ -133,7 +134,7 @@ int ca_append_8bit(const void* key, const void* value, int64_t seq_stride, int64
   if (!page_ok(page)) return CA_EPAGE;
   if (!sizes_ok(batch, heads, num_blocks, table_width, n_new) || total_new < 0) return CA_ESHAPE;
   if (batch == 0 || n_new == 0 || (cu_new && total_new == 0)) return CA_OK;
-  if (!k_scale || !v_scale) return CA_ENULL;
+  if (num_blocks && (!k_scale || !v_scale)) return CA_ENULL;
   if (!aligned(k_scale, 4) || !aligned(v_scale, 4)) return CA_ELAYOUT;
   ca::AppendParams prm{};
   bool vec16;
@@ -168,8 +169,8 @@ int ca_decode_split(const void* q, int64_t q_stride, void* k_cache, void* v_cach
   if (table_width * page > 0x7fffffffLL) return CA_ESHAPE;
   if ((k_new == nullptr) != (v_new == nullptr) || (k_new == nullptr) != (n_new == 0)) return CA_ESHAPE;
   if (batch == 0) return CA_OK;
-  if (!q || !k_cache || !v_cache || !lens || !page_table || !out || !workspace) return CA_ENULL;
-  if (eight && (!k_scale || !v_scale)) return CA_ENULL;
+  if (!q || !lens || !out || !workspace || (table_width && !page_table)) return CA_ENULL;
+  if (num_blocks && (!k_cache || !v_cache || (eight && (!k_scale || !v_scale)))) return CA_ENULL;
   if (q_stride < heads * head_dim && batch > 1) return CA_ELAYOUT;
   const size_t es = elem_size(q_dtype);
   if (!aligned(q, es) || !aligned(out, 2 * es) || !aligned(lse, 4) || !aligned(k_cache, 16) ||

@@ -354,6 +354,133 @@ def test_decode_graphs_and_streams():
             assert torch.equal(out, call())
 
 
+def test_decode_graphs_of_one_stream_on_two():
+    """Two graphs captured on the same stream, replayed at once on two others: each has buffers of its own."""
+    C = api()
+    s = torch.cuda.Stream()
+    runs = []
+    for x in range(2):
+        pc = S.Paged("8bit", [3000, 70, 900], 2, 64, 16, BF16, seed=20 + x)
+        q = torch.randn(3, 1, 8, 64, generator=torch.Generator().manual_seed(x)).bfloat16().to(DEV)
+        call = lambda pc=pc, q=q: C.flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L,  # noqa
+                                                            page_table=pc.bt, window_size=(2000, 0), sink_tokens=5,
+                                                            **pc.opts())
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = call()
+        runs.append((graph, out, call, torch.cuda.Stream()))  # (the graph reads what `call` holds)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, _, _, stream in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, call, _ in runs:
+        assert torch.equal(out, call())
+
+
+def test_offsets_past_32_bits():
+    """Blocks more than 2^32 bytes into 8-bit caches: written, read, copied and packed in place."""
+    C = api()
+    blocks, hk, page, d = 280000, 8, 16, 128  # 4.6e9 bytes a side
+    kc, vc = (torch.zeros(blocks, hk, page, d, dtype=torch.uint8, device=DEV).view(S.F8) for _ in range(2))
+    ks, vs = (torch.zeros(blocks, hk, device=DEV) for _ in range(2))
+    g = torch.Generator().manual_seed(0)
+    ids = [blocks - 1, 3, blocks - 7]
+    table = torch.tensor([ids], dtype=torch.int32, device=DEV)
+    L = torch.zeros(1, dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(1, 40, hk, d, generator=g).bfloat16().to(DEV) for _ in range(2))
+    C.append_quantized(k, v, kc, vc, ks, vs, L, table)
+    small = [t[ids].contiguous() for t in (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)]
+    q = torch.randn(1, 1, 16, d, generator=g).bfloat16().to(DEV)
+    want = C.flash_attn_with_kvcache(q, small[0].view(S.F8), small[1].view(S.F8), cache_seqlens=40,
+                                     page_table=torch.tensor([[0, 1, 2]], dtype=torch.int32, device=DEV),
+                                     k_descale=small[2], v_descale=small[3])
+    ref, *_ = S.attention(q[0, 0, :2].double().cpu(), k[0, :, 0].double().cpu(), v[0, :, 0].double().cpu(),
+                          torch.ones(2, 40, dtype=torch.bool), d ** -0.5)
+    assert (want[0, 0, :2].double().cpu() - ref).abs().max() < 0.3  # the tokens, to 8 bits
+    caches = [kc, vc, ks, vs]
+    for step in range(3):
+        got = C.flash_attn_with_kvcache(q, kc, vc, cache_seqlens=40, page_table=table, k_descale=ks, v_descale=vs)
+        assert torch.equal(got, want), step
+        if step == 0:
+            C.copy_blocks(caches, torch.tensor([[blocks - 1, 100], [3, blocks - 2], [blocks - 7, blocks - 9]], device=DEV))
+            table = torch.tensor([[100, blocks - 2, blocks - 9]], dtype=torch.int32, device=DEV)
+        elif step == 1:
+            table, used = C.compact_blocks(caches, table, torch.tensor([40], dtype=torch.int32, device=DEV), page)
+            assert used.tolist() == [3] and sorted(table[0].tolist()) == [0, 1, 2]
+    assert status() == 0
+
+
+def test_strides_of_sizes_of_one():
+    """One head, one token, one sequence: such a dim's stride may be anything."""
+    C = api()
+    g = torch.Generator().manual_seed(3)
+    pc = S.Paged("8bit", [20], 1, 64, 16, BF16, seed=2, room=1)
+    for c in (pc.k_cache, pc.v_cache):
+        u = c.view(torch.uint8)
+        u[(u & 0x7f) == 0x7f] = 0
+    k, v = (torch.randn(1, 1, 1, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    q = torch.randn(1, 1, 1, 64, generator=g).bfloat16().to(DEV)
+    want = C.flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, k=k, v=v, cache_seqlens=pc.L, page_table=pc.bt,
+                                     **pc.opts())
+    odd = lambda t: torch.as_strided(t, (1, 1, 1, 64), (3, 7, 5, 1))  # noqa: E731
+    got = C.flash_attn_with_kvcache(odd(q), pc.k_cache, pc.v_cache, k=odd(k), v=odd(v), cache_seqlens=pc.L,
+                                    page_table=pc.bt, **pc.opts())
+    assert torch.equal(got, want)
+    before = [bytes_of(c) for c in (pc.k_cache, pc.v_cache)]
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    for key, value in ((odd(k)[0], odd(v)[0]), (k[0], v[0])):
+        C.append_quantized(key, value, pc.k_cache, pc.v_cache, pc.k_scale, pc.v_scale, pc.L, pc.bt, cu, 1)
+        assert all(torch.equal(bytes_of(c), b) for c, b in zip((pc.k_cache, pc.v_cache), before))
+    assert torch.equal(want, C.flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L + 1,
+                                                       page_table=pc.bt, **pc.opts()))
+
+
+def test_caches_at_an_odd_address_are_refused():
+    C = api()
+    raw = torch.zeros(4 * 16 * 64 + 16, dtype=torch.uint8, device=DEV)
+    off = raw[4:4 + 4 * 16 * 64].view(4, 1, 16, 64).view(S.F8)
+    one = torch.ones(4, 1, device=DEV)
+    q = torch.zeros(1, 1, 1, 64, dtype=BF16, device=DEV)
+    bt = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="16 bytes"):
+        C.flash_attn_with_kvcache(q, off, off, cache_seqlens=3, page_table=bt, k_descale=one, v_descale=one)
+    with pytest.raises(ValueError, match="16 bytes"):
+        C.append_quantized(q, q, off, off, one, one.clone(), torch.zeros(1, dtype=torch.int32, device=DEV), bt)
+
+
+def test_empty_calls():
+    """No sequences, no new tokens, tables of no pages."""
+    C = api()
+    kc, vc, ks, vs = empty_8bit(4, 2, 16, 64, 0)
+    no = torch.zeros(0, dtype=torch.int32, device=DEV)
+    q0 = torch.zeros(0, 1, 4, 64, dtype=BF16, device=DEV)
+    out, lse = C.flash_attn_with_kvcache(q0, kc, vc, cache_seqlens=no, page_table=no.view(0, 3), k_descale=ks,
+                                         v_descale=vs, return_softmax_lse=True)
+    assert out.shape == q0.shape and lse.shape == (0, 4, 1)
+    q = torch.ones(2, 1, 4, 64, dtype=BF16, device=DEV)
+    two = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for table in (two.view(2, 1), no.view(2, 0)):
+        new = torch.zeros(2, 0, 2, 64, dtype=BF16, device=DEV)
+        out = C.flash_attn_with_kvcache(q, kc, vc, k=new, v=new, cache_seqlens=two, page_table=table, k_descale=ks,
+                                        v_descale=vs)
+        assert (out == 0).all()
+        C.append_quantized(new, new, kc, vc, ks, vs, two, table)
+    C.append_quantized(q0[:, 0, :2], q0[:, 0, :2], kc, vc, ks, vs, two, two.view(2, 1),
+                       torch.zeros(3, dtype=torch.int32, device=DEV))
+    pool = empty_8bit(0, 2, 16, 64, 0)
+    out = C.flash_attn_with_kvcache(q, *pool[:2], cache_seqlens=two, page_table=two.view(2, 1), k_descale=pool[2],
+                                    v_descale=pool[3])
+    assert (out == 0).all() and (ks == 0).all() and status() == 0
+    new, used = C.compact_blocks([kc], no.view(2, 0), two, 16)
+    assert new.shape == (2, 0) and used.tolist() == [0]
+
+
 # ------------------------------------------------------------------ prefill --
 def check_prefill(out, lse, q, k, v, left, right, sinks, causal, scale=None):
     """One sequence: out [lq, h, d] against the definition. Weights enter the bf16 kernel's second product rounded to
