@@ -89,6 +89,7 @@ __device__ __forceinline__ void copy_group(const CopyParams& p, char* base, int 
 }
 
 __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const __grid_constant__ CopyParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // behind a plan: its moves are written
   const long long n = p.pairs ? p.n : __ldg(p.count);
   const int small = p.tensors - p.large;
   const long long groups = (n + kCopyGroup - 1) / kCopyGroup;
@@ -178,6 +179,7 @@ __device__ __forceinline__ int plan_scan(int x, int* wsum, int* total) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint32_t plan_bits[];  // one bit per block
   __shared__ int wsum[32];
   const int words = (int)((p.num_blocks + 31) / 32);

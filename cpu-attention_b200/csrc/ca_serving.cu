@@ -291,9 +291,18 @@ int ca_compact_blocks(void* const* base, const int64_t* block_bytes, int64_t ten
     copy_params(&prm, base, block_bytes, first, tensors, num_blocks, status);
     prm.moves = p.moves;
     prm.count = p.count;
-    // (how many blocks move is known on the device only: 8 CTAs an SM share them)
-    ca::copy_blocks_kernel<<<(unsigned)(8 * sms), ca::kCopyThreads, 0, s>>>(prm);
-    e = cudaGetLastError();
+    // (how many blocks move is known on the device only: 8 CTAs an SM share them.
+    // The first launch may come up while the plan is made.)
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(8 * sms));
+    cfg.blockDim = dim3(ca::kCopyThreads);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = first == 0 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, ca::copy_blocks_kernel, prm);
     if (e != cudaSuccess) return ca::host_cuda_fail(e, "compact copy launch");
   }
   return CA_OK;

@@ -87,7 +87,6 @@ cudaError_t split_launch(const SplitCall& c, int sms, int device, cudaStream_t s
     prm.left = c.left < 0 ? -1 : (int)std::min<long long>(c.left, 0x7fffffff);
     prm.sinks = (int)std::min<long long>(c.sinks, 0x7fffff00);
     prm.c = c.c;
-    prm.min_chunk = 2;
     prm.q_vec = (reinterpret_cast<uintptr_t>(prm.q) % 16 == 0) && (c.q_stride * es) % 16 == 0;
     prm.partial = static_cast<float*>(c.workspace);
     prm.meta = reinterpret_cast<int*>(prm.partial + (size_t)ctas * 2 * piece_bytes(c.head_dim) / 4);

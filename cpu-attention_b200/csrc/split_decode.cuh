@@ -86,7 +86,6 @@ struct SplitParams {
   int page;
   int left, sinks;  // left < 0: no window
   float c;          // softmax_scale * log2(e)
-  int min_chunk;    // units a warp takes at least
   int q_vec;        // q's rows are 16-byte aligned
   float* partial;   // pieces [CTAs][2] of items cut by a CTA boundary
   int* meta;        // [CTAs][4]: the item CTA c leaves unfinished {sequence, item, last CTA, 1}, or {.., 0}
@@ -1111,7 +1110,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitCtasPerSm)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long total = split_units(prefix, p.B, p.IH);
   const long long warps = (long long)gridDim.x * kSplitWarps;
-  const long long chunk = max((long long)p.min_chunk, (total + warps - 1) / warps);
+  const long long chunk = max(1LL, (total + warps - 1) / warps);
   const long long w0 = min(total, ((long long)blockIdx.x * kSplitWarps + warp) * chunk);
   const long long w1 = min(total, w0 + chunk);
 
