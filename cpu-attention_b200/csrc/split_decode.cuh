@@ -11,19 +11,28 @@
 // [dim] for both (codes are read as matrix fragments, no transpose is needed);
 // float caches keep the layout of store.cuh.
 //
-// What bounds it: HBM. A 16-token tile of one KV head is 4 KiB of codes at
-// head_dim 128 (8 KiB bf16, 16 KiB fp32), read once for up to 8 query rows.
+// What bounds it: HBM. 16 tokens of one KV head are 4 KiB of codes at head_dim
+// 128 (8 KiB bf16, 16 KiB fp32), read once for up to 8 query rows. Measured
+// (one B200, device time, inputs larger than L2): bf16 behind a window of 4096,
+// 64 sequences, 32 / 8 heads: 155 us for 1.00 GB (6.5 TB/s, 98% of the measured
+// copy rate); 8-bit, 64 sequences to 8191 tokens, 64 / 8 heads: 94 us for 0.54
+// GB (5.7 TB/s); 32 sequences of 16 heads to 2047 tokens: 33 us for 136 MB, of
+// which about 6 us pass before the first tile is in (lengths, block ids and
+// scales, tiles: round trips that wait for one another) and 5 us behind the
+// last one (the join); 8-bit tiles are then bound by latency of the chain
+// widen, multiply, weigh (40% of issue slots used), not by HBM.
 //
 // Work: the visible tokens of every item (sequence, KV head, up to 8 of its
-// query heads) are cut into tiles of 16 tokens; pages between the first tokens
-// and the window are neither read nor looked up, so their page-table entries
-// may be anything. All tiles are numbered in (sequence, head, token) order and
-// every warp of the grid takes an equal, contiguous run of them, so lengths
-// need not be known on the host and ragged batches stay balanced. An item cut
-// by a warp boundary leaves its (m, l, O) in shared memory, where its CTA joins
-// the pieces in tile order; one cut by a CTA boundary goes through a small
-// global buffer and split_merge_kernel, also in order. The result does not
-// depend on timing, and nothing is kept between calls.
+// query heads) are cut into tiles of 16 tokens (more for small head_dims); pages
+// between the first tokens and the window are neither read nor looked up, so
+// their page-table entries may be anything. All tiles are numbered in (sequence,
+// head, token) order and every warp of the grid takes an equal, contiguous share
+// of them (an item counts two tiles more than it has, for its queries, its join
+// and its output), so lengths need not be known on the host and ragged batches
+// stay balanced. An item cut by a warp boundary leaves its (m, l, O) in shared
+// memory, where its CTA joins the pieces in tile order; one cut by a CTA
+// boundary goes through a small global buffer and split_merge_kernel, also in
+// order. The result does not depend on timing, and nothing is kept between calls.
 //
 // A tile in a warp (lane = 4 * g + t), MMA kinds (8-bit and bf16 caches):
 //   S^T = K Q^T   m16n8k16: rows = keys, columns = query rows. The lane's K
@@ -42,8 +51,14 @@
 //
 // Loads of tile n+1 are issued as soon as the registers of tile n are free: 12
 // warps an SM with a tile each in flight are 48 KiB, about twice what HBM's
-// latency asks for. mma.sync and not tcgen05: a tcgen05 tile has at least 64
-// rows, of which at most 8 (16) query rows would be used.
+// latency asks for; 8-bit tiles are called into L2 one tile earlier still (-8%;
+// four tiles earlier: +4%, eight: +17%). Measured against this (8-bit grouped,
+// 96 us then): cp.async into shared memory with four tiles ahead 132 us, TMA
+// tiles swizzled for conflict-free fragment loads 96 us, two tiles ahead in
+// registers 98 us, the next tile's scores before this one's weights 117 us, 8
+// warps an SM 112 us, 16 warps 99 us (spills). mma.sync with e4m3 operands
+// widens inside on sm_100a: 134 us. mma.sync and not tcgen05: a tcgen05 tile has
+// at least 64 rows, of which at most 8 (16) query rows would be used.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -58,13 +73,16 @@ constexpr int kSplitWarps = 6;        // warps per CTA
 constexpr int kSplitCtasPerSm = 2;    // CTAs per SM
 constexpr int kSplitTile = 16;        // tokens per tile
 constexpr int kSplitMaxBatch = 1024;  // sequences per launch (their tile counts sit in shared memory)
-constexpr int kSplitRing = 16384;     // bytes of tiles a warp has in flight
+constexpr int kSplitRing = 16384;     // fp32 caches: bytes of tiles a warp has in flight
 constexpr int kSplitMeta = 64;        // tiles whose places a warp keeps
 constexpr int kSplitAhead = 2;        // tiles ahead whose lines are brought to L2 (at most 16)
 // Weights are kept as 2^(x - m + kUp), m a reference that a column's largest x
 // may pass by kSlack before it moves (a vote per tile, no reduction): up to 2^14
 // for f16, whose smallest step is then 2^-30 of the reference's weight.
 constexpr float kUp = 6.f, kSlack = 8.f;
+// Shares of an item's pieces that a join takes side by side. 2 (blocks of 512
+// threads, all resident at once) against 4: 32.5 and 35 us with two or three
+// pieces an item (32 x 16 heads), 57 and 55 us with 37 (one long sequence).
 constexpr int kSplitMergeShares = 2;
 
 struct SplitParams {
@@ -777,9 +795,8 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
         }
       }
     } else {
-      float s2[2][4];  // two chains
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s2[0][r] = s2[1][r] = 0.f;
+      for (int r = 0; r < 4; ++r) s[r] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < C::NM; ++kk) {
         uint32_t f[4];
@@ -796,10 +813,8 @@ struct SplitWarp : SplitWalk<KIND, QT, E> {
           f[3] = kr[4 * kk + 3];
         }
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) split_mma<kPBf16>(s2[kk & 1], f, q[x][kk][0], q[x][kk][1]);
+        for (int x = 0; x < NQ; ++x) split_mma<kPBf16>(s, f, q[x][kk][0], q[x][kk][1]);
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] = s2[0][r] + s2[1][r];
     }
   }
 
@@ -1043,8 +1058,8 @@ __host__ __device__ constexpr int split_smem_fixed() {
   return kSplitWarps * (SplitRing<KIND, E>::kWarpBytes + 2 * SplitCfg<KIND, E>::kPieceFloats * 4) + kSplitWarps * 2 * (int)sizeof(SplitPiece) + 128;
 }
 
-// Work is shared out in units: an item is kSplitItemUnits and one for each of
-// its tiles. Where unit u of the launch lies: the tile at or after it.
+// Work is shared out in units: an item is kSplitItemUnits (2 and 3: the same; 1:
+// +7% on 32 x 16 heads) and one for each of its tiles. Where unit u of the launch lies: the tile at or after it.
 constexpr int kSplitItemUnits = 2;
 
 struct SplitSpot {

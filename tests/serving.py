@@ -172,13 +172,11 @@ def check_decode(out, lse, q, pc, heads, scale=None, lens=None):
     scale = d ** -0.5 if scale is None else scale
     group = heads // kv
     fp32 = q.dtype == torch.float32
-    # 8-bit caches under bf16 queries: a weight is two e4m3 values, the second the first's rest: |w - w1| <= 2^-4 w
-    # (half a step of e4m3), rounded again to half a step of itself: 2^-8 w. Below e4m3's normal range the rest's half
-    # step is absolute: 2^-10 / 16 where the tile's largest weight is 2^7 or more, 2^-21 of it; over the 32 keys of
-    # each tile, and the tiles' largest weights sum to 1 at most: 32 * 2^-21 * max |v| in all.
-    # Under fp32 queries it is two f16 values: 2^-11 squared.
-    eight = pc.kind == "8bit" and not fp32
-    weight = {"8bit": 2.0 ** -22 if fp32 else 2.0 ** -8, "bf16": 2.0 ** -16, "fp32": 0.0}[pc.kind]
+    # 8-bit caches under bf16 queries: a weight is one f16 value, half a step 2^-11. The largest weight * scale is 2^6 or
+    # more, so below f16's normal range the half step 2^-25 is 2^-31 of it: keys * 2^-31 * max |v| in all. Under fp32
+    # queries it is two f16 values: 2^-11 squared. bf16 caches: two bf16 values, 2^-8 squared.
+    eight = pc.kind == "8bit"
+    weight = {"8bit": 2.0 ** -22 if fp32 else 2.0 ** -11, "bf16": 2.0 ** -16, "fp32": 0.0}[pc.kind]
     query = 2.0 ** -22 if pc.kind == "8bit" else 0.0
     got = out.double().cpu()
     for i, n in enumerate(pc.lens if lens is None else lens):
@@ -189,7 +187,7 @@ def check_decode(out, lse, q, pc, heads, scale=None, lens=None):
             ref, z, spread, top = attention(qq, k, v, torch.ones(group, len(pos), dtype=torch.bool), scale)
             tol = bound(ref, spread, top, d, len(pos), q.dtype, weight, query)
             if eight and len(pos):
-                tol = tol + 2.0 ** -16 * v.abs().amax(0)
+                tol = tol + len(pos) * 2.0 ** -31 * v.abs().amax(0)
             err = (got[i, 0, h * group:(h + 1) * group] - ref).abs()
             assert (err <= tol).all(), (i, h, err.max().item(), (err / tol).max().item())
             if lse is not None:

@@ -735,7 +735,7 @@ def test_serving_run(kind):
                 # values by 2^-4 of themselves plus two units of the smallest step of a block of N(0, 1) values
                 eight = kind == "8bit"
                 shift = top * 1.1 * 2 ** -4 if eight else torch.zeros_like(top)
-                tol = S.bound(ref, spread, top, d, len(pos), BF16, 2.0 ** -8 if eight else 2.0 ** -16)
+                tol = S.bound(ref, spread, top, d, len(pos), BF16, 2.0 ** -11 if eight else 2.0 ** -16)
                 tol = tol + (spread + 0.05) * (torch.expm1(2 * shift)[:, None] + (2 ** -4 if eight else 0)) + 1e-3
                 err = (out[x, 0, a * 4:(a + 1) * 4].double().cpu() - ref).abs()
                 assert (err <= tol).all(), (step, i, err.max().item())
