@@ -107,7 +107,7 @@ def build_fastpath(force=False, verbose=False):
     cmd = [gxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_EXTENSION_NAME=_fastpath", "-DTORCH_API_INCLUDE_EXTENSION_H",
            *[f"-I{d}" for d in incs], FAST_SRC, "-o", out + ".tmp",
-           *[f"-L{d}" for d in libdirs], "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           *[f"-L{d}" for d in libdirs], "-lc10", "-lc10_cuda", "-lcudart", "-ltorch", "-ltorch_cpu", "-ltorch_python",
            f"-L{os.path.dirname(OUT)}", "-lca_b200", "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in libdirs]]
     if verbose:
         print(" ".join(cmd), flush=True)

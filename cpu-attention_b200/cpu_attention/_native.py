@@ -293,9 +293,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_TENSORS = {torch.Tensor}
+_TENSORS_OR_NONE = {torch.Tensor, type(None)}
+
+
 def _checked(device, out):
     """``out``, once CHECK mode has seen the status of what was launched."""
-    if out is not None and K.CHECK:
+    if K.CHECK and out is not None:
         K.raise_status(device, K.current_stream(device))
     return out
 
@@ -308,8 +312,8 @@ def decode_split(rt, q, k_cache, v_cache, k, v, k_scale, v_scale, lens, page_tab
     appended at ``lens`` first. Returns the output, or None."""
     del rt
     fast = K.fastpath()
-    if (fast is not None and _plain_tensors(q, k_cache, v_cache, lens, page_table)
-            and _plain_or_none(k, v, k_scale, v_scale, lse)):
+    if (fast is not None and {type(q), type(k_cache), type(v_cache), type(lens), type(page_table)} == _TENSORS
+            and {type(k), type(v), type(k_scale), type(v_scale), type(lse)} <= _TENSORS_OR_NONE):
         return _checked(q.device, fast.decode_split(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, page_table,
                                                     left, sinks, None if scale is None else float(scale), lse))
     dev = _cuda(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, page_table, lse)
@@ -363,8 +367,8 @@ def append_8bit(rt, key, value, k_cache, v_cache, k_scale, v_scale, lens, page_t
     None."""
     del rt
     fast = K.fastpath()
-    if (fast is not None and _plain_tensors(key, value, k_cache, v_cache, k_scale, v_scale, lens, page_table)
-            and _plain_or_none(cu)):
+    if (fast is not None and {type(key), type(value), type(k_cache), type(v_cache), type(k_scale), type(v_scale),
+                              type(lens), type(page_table)} == _TENSORS and type(cu) in _TENSORS_OR_NONE):
         return _checked(key.device, fast.append_8bit(key, value, k_cache, v_cache, k_scale, v_scale, lens, page_table,
                                                      cu, max_new))
     dev = _cuda(key, value, k_cache, v_cache, k_scale, v_scale, lens, page_table, cu)

@@ -196,6 +196,12 @@ def flash_attn_with_kvcache(
 
 def _window(window_size, sink_tokens):
     """(left, right, sinks) of a window, checked."""
+    if type(window_size) is tuple and len(window_size) == 2 and type(sink_tokens) is int:
+        # (the usual case: an engine calls this once per layer and token)
+        left, right = window_size
+        if type(left) is int and type(right) is int and -1 <= left < 1 << 30 and -1 <= right < 1 << 30 \
+                and 0 <= sink_tokens < 1 << 30:
+            return left, right, sink_tokens
     try:
         left, right = (int(x) for x in window_size)
         sinks = int(sink_tokens)

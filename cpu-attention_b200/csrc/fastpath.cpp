@@ -14,6 +14,7 @@
 
 #include <torch/extension.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -43,6 +44,20 @@ at::Tensor workspace(int64_t device, uintptr_t stream, int64_t nbytes) {
   const int64_t size = std::max({nbytes, kMinWorkspace, grown});
   at::Tensor ws = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
   g_ws[key] = ws;
+  return ws;
+}
+
+// The split decode's buffer: one per (device, stream) -- calls on a stream are
+// ordered, and nothing in it outlives a call -- but one of its own for every
+// captured call, since graphs may be replayed side by side.
+std::map<std::pair<int, uintptr_t>, at::Tensor> g_split_ws;
+at::Tensor split_workspace(int64_t device, uintptr_t stream, int64_t nbytes) {
+  const auto options = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return at::empty({nbytes}, options);
+  std::lock_guard<std::mutex> lock(g_ws_mutex);
+  at::Tensor& ws = g_split_ws[std::make_pair((int)device, stream)];
+  if (!ws.defined() || ws.numel() < nbytes) ws = at::empty({nbytes}, options);
   return ws;
 }
 
@@ -265,9 +280,7 @@ py::object decode_split(const at::Tensor& q, const at::Tensor& kc, const at::Ten
   const c10::cuda::CUDAGuard guard(device);
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   const size_t need = ca_decode_split_workspace_bytes(hd, dev);
-  // its own buffer for every call: calls on other streams, and captured ones
-  // replayed beside others, share nothing
-  at::Tensor scratch = at::empty({(int64_t)need}, q.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor scratch = split_workspace(dev, (uintptr_t)stream, (int64_t)need);
   at::Tensor ws = workspace(dev, (uintptr_t)stream, 0);
   const bool fresh = n_new > 0;
   const int rc = ca_decode_split(
@@ -276,7 +289,8 @@ py::object decode_split(const at::Tensor& q, const at::Tensor& kc, const at::Ten
       fresh ? v->data_ptr() : nullptr, fresh ? k->stride(0) : 0, fresh ? k->stride(1) : 0, n_new,
       lens.data_ptr<int32_t>(), pt.data_ptr<int32_t>(), pt.size(1), out.data_ptr(),
       lse ? lse->data_ptr<float>() : nullptr, b, heads, kvh, hd, page, dt, eight ? CA_DTYPE_E4M3 : dt, left, sinks,
-      scale ? (float)*scale : std::nanf(""), scratch.data_ptr(), need, static_cast<int32_t*>(ws.data_ptr()), stream);
+      scale ? (float)*scale : std::nanf(""), scratch.data_ptr(), (size_t)scratch.numel(),
+      static_cast<int32_t*>(ws.data_ptr()), stream);
   if (rc == CA_ECUDA) throw std::runtime_error(std::string("cpu_attention: ") + ca_last_cuda_error());
   if (rc != CA_OK) return py::none();
   return py::cast(out);
