@@ -73,8 +73,8 @@ __device__ __forceinline__ bool copy_pair(const CopyParams& p, long long pair, l
       return false;
     }
   } else {
-    *src = __ldg(p.moves + 2 * pair);
-    *dst = __ldg(p.moves + 2 * pair + 1);
+    *src = __ldcg(p.moves + 2 * pair);  // (the plan may still write them as the launch begins)
+    *dst = __ldcg(p.moves + 2 * pair + 1);
   }
   return *src != *dst;
 }
@@ -92,7 +92,7 @@ __device__ __forceinline__ void copy_group(const CopyParams& p, char* base, int 
 
 __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const __grid_constant__ CopyParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // behind a plan: its moves are written
-  const long long n = p.pairs ? p.n : __ldg(p.count);
+  const long long n = p.pairs ? p.n : __ldcg(p.count);
   const int small = p.tensors - p.large;
   const long long groups = (n + kCopyGroup - 1) / kCopyGroup;
   // units: a pair of a tensor with large blocks, then a group of pairs of one with small blocks

@@ -209,7 +209,8 @@ __device__ __forceinline__ void split_copy(uint32_t dst, const void* src, bool o
     asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
                  : "memory");
 }
-// The same to registers; lines are read once per item, past L1.
+// The same to registers; lines are read once per item, past L1. (Not by the
+// read-only path: an append may still write the cache as the launch begins.)
 template <int BYTES, bool FULL>
 __device__ __forceinline__ void split_load(uint32_t* r, const void* p, bool on) {
   if constexpr (!FULL) {
@@ -218,13 +219,13 @@ __device__ __forceinline__ void split_load(uint32_t* r, const void* p, bool on) 
     if (!on) return;
   }
   if constexpr (BYTES == 16)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "l"(p));
   else if constexpr (BYTES == 8)
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
   else
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
 }
 __device__ __forceinline__ void split_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -467,8 +468,8 @@ struct SplitWalk {
         if (p.status) atomicOr(p.status, CA_STATUS_TABLE);
         m_mask &= ~0xffffu;
       } else if constexpr (C::k8) {
-        m_sk = __ldg(p.ks + (long long)m_id * p.Hk + m_kvh);
-        m_sv = __ldg(p.vs + (long long)m_id * p.Hk + m_kvh);
+        m_sk = __ldcg(p.ks + (long long)m_id * p.Hk + m_kvh);
+        m_sv = __ldcg(p.vs + (long long)m_id * p.Hk + m_kvh);
       }
     }
   }
