@@ -15,10 +15,9 @@
 // One warp owns a (sequence, touched page, head) of K or of V: it is the only
 // writer of that block and scale, so there are no atomics and the result does
 // not depend on order. Bound by HBM (2 bytes read and 1 written per value at
-// bf16) for prompts: 24.6k tokens of 16 heads of 128 dims, 302 MB, in 58 us (5.2
-// TB/s, 79% of the measured copy rate; half of the issue slots are used). One
-// token per sequence is a launch and three loads that wait for one another
-// (length, block id, scale): 2.6 us.
+// bf16) for prompts: 24.6k tokens of 16 heads of 128 dims, 302 MB, in 49 us (6.2
+// TB/s, 94% of the measured copy rate). One token per sequence is a launch and
+// three loads that wait for one another (length, block id, scale): 2.8 us.
 //
 // append_rows_kernel: the same places in a float cache, bit-exact (the layout
 // of store.cuh), any number of tokens per sequence.
@@ -126,6 +125,11 @@ __device__ __forceinline__ void append_load(float (&x)[VEC], const T* p) {
 }
 
 constexpr int kAppendWarps = 4;
+// 8 CTAs an SM (64 registers, nothing of bf16 spilled) keep enough loads in flight:
+// prompts 49.1 us; 6 CTAs 55.1, as many as the registers would leave (5) 58.4,
+// 10 (held vectors spill) 55.2. One token a sequence does not fill an SM and loses
+// 0.1 us to the tighter schedule.
+constexpr int kAppendCtas = 8;
 constexpr int kAppendHeld = 8;  // vectors a lane keeps between the maximum and the codes
 
 // The largest magnitude of a vector's values and `top`, as bits (two bf16 at a
@@ -207,7 +211,7 @@ __device__ __forceinline__ int append_sequence(const AppendParams& p, long long 
 // The rows are loaded before the block id is known; a 16-token page of head_dim
 // 128 (bf16) stays in registers, so new tokens are read once.
 template <typename T, int E, bool VEC16>
-__global__ void __launch_bounds__(32 * kAppendWarps) append_8bit_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, kAppendCtas) append_8bit_kernel(const __grid_constant__ AppendParams p) {
   constexpr int VEC = VEC16 ? 16 / (int)sizeof(T) : 1;
   constexpr int PER_ROW = E / VEC;                            // vectors of a row
   constexpr int LANES = PER_ROW < 32 ? PER_ROW : 32;          // lanes that share a row
