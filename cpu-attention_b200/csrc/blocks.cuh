@@ -3,8 +3,9 @@
 //
 // copy_blocks_kernel: pair (src, dst) of every tensor [num_blocks, ...]; a CTA
 // copies one block of one tensor, or (blocks up to 1 KiB: scales) 64 pairs of it.
-// Bound by HBM: each byte read and written once; 8 words a thread in flight. 65
-// blocks of 48 tensors (204 MB both ways) in 33 us, 6.1 TB/s.
+// Bound by HBM: each byte read and written once; 8 words a thread in flight
+// (4 at twice the warps: 44 us; 512 threads: 48 us; 128: 34 us). 65 blocks of 48
+// tensors (204 MB both ways) in 33 us, 6.1 TB/s.
 //
 // compact_plan_kernel (one CTA): with U the blocks that the page table's rows
 // use and n = |U|, the k-th smallest member of U that is >= n goes to the k-th
@@ -12,7 +13,8 @@
 // the destinations are disjoint, so the copies need no order. A block
 // several rows share moves once. U is a bitmap in shared memory; ranks are
 // prefix sums of its population counts. A pool of 2111 blocks is planned in 9.5
-// us; with its moves (24 8-bit caches and their scales, 387 MB) 69 us.
+// us; with its moves (24 8-bit caches and their scales, 387 MB) 70 us (a move's ids
+// loaded only once the last one's bytes are written: 77 us).
 #pragma once
 
 #include "common.cuh"
@@ -22,6 +24,7 @@ namespace ca {
 constexpr int kCopyTensors = 128;  // tensors per launch
 constexpr int kCopyThreads = 256;
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanHeld = 4;  // table entries a thread reads once; those behind are read twice
 constexpr int kPlanMaxBlocks = 1 << 20;  // a 128 KiB bitmap
 
 constexpr int kCopySmall = 1024;  // bytes up to which a CTA takes kCopyGroup pairs of a tensor at a time
@@ -62,21 +65,28 @@ __device__ __forceinline__ void copy_words(char* dst, const char* src, long long
   }
 }
 
-// (src, dst) of a pair; false when it is left out.
-__device__ __forceinline__ bool copy_pair(const CopyParams& p, long long pair, long long* src, long long* dst) {
+struct CopyPair {
+  long long src, dst;
+};
+__device__ __forceinline__ CopyPair copy_pair(const CopyParams& p, long long pair) {
+  CopyPair c;
   if (p.pairs) {
-    *src = __ldg(p.pairs + 2 * pair);
-    *dst = __ldg(p.pairs + 2 * pair + 1);
-    if (*src < 0 || *dst < 0) return false;  // padding
-    if (*src >= p.num_blocks || *dst >= p.num_blocks) {
-      if (p.status) atomicOr(p.status, CA_STATUS_SLOT);
-      return false;
-    }
-  } else {
-    *src = __ldcg(p.moves + 2 * pair);  // (the plan may still write them as the launch begins)
-    *dst = __ldcg(p.moves + 2 * pair + 1);
+    c.src = __ldg(p.pairs + 2 * pair);
+    c.dst = __ldg(p.pairs + 2 * pair + 1);
+  } else {  // (the plan may still write them as the launch begins: not by the read-only path)
+    c.src = p.moves[2 * pair];
+    c.dst = p.moves[2 * pair + 1];
   }
-  return *src != *dst;
+  return c;
+}
+// Whether it is copied: negative ids are padding, one beyond the pool is flagged.
+__device__ __forceinline__ bool copy_counts(const CopyParams& p, const CopyPair& c) {
+  if (c.src < 0 || c.dst < 0) return false;
+  if (c.src >= p.num_blocks || c.dst >= p.num_blocks) {
+    if (p.status) atomicOr(p.status, CA_STATUS_SLOT);
+    return false;
+  }
+  return c.src != c.dst;
 }
 
 template <typename W>
@@ -84,9 +94,9 @@ __device__ __forceinline__ void copy_group(const CopyParams& p, char* base, int 
   const int per = bytes / (int)sizeof(W);
   for (int x = threadIdx.x; x < pairs * per; x += kCopyThreads) {
     const int k = x / per, w = x - k * per;
-    long long src, dst;
-    if (!copy_pair(p, first + k, &src, &dst)) continue;
-    reinterpret_cast<W*>(base + dst * bytes)[w] = reinterpret_cast<const W*>(base + src * bytes)[w];
+    const CopyPair c = copy_pair(p, first + k);
+    if (!copy_counts(p, c)) continue;
+    reinterpret_cast<W*>(base + c.dst * bytes)[w] = reinterpret_cast<const W*>(base + c.src * bytes)[w];
   }
 }
 
@@ -95,38 +105,42 @@ __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const __grid_
   const long long n = p.pairs ? p.n : __ldcg(p.count);
   const int small = p.tensors - p.large;
   const long long groups = (n + kCopyGroup - 1) / kCopyGroup;
-  // units: a pair of a tensor with large blocks, then a group of pairs of one with small blocks
-  for (long long u = blockIdx.x; u < n * p.large + groups * small; u += gridDim.x) {
-    if (u < n * p.large) {
-      const unsigned long long pair = u <= 0xffffffffLL ? (unsigned)u / (unsigned)p.large : u / p.large;
-      const int t = (int)(u - pair * p.large);
-      long long src, dst;
-      if (!copy_pair(p, pair, &src, &dst)) continue;
-      const long long bytes = p.bytes[t];
-      const char* s = p.base[t] + src * bytes;
-      char* d = p.base[t] + dst * bytes;
-      const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
-      if ((at & 15) == 0)
-        copy_words<uint4>(d, s, bytes);
-      else if ((at & 3) == 0)
-        copy_words<uint32_t>(d, s, bytes);
-      else
-        copy_words<uint8_t>(d, s, bytes);
-    } else {
-      const long long v = u - n * p.large;
-      const long long group = v / small;
-      const int t = p.large + (int)(v - group * small);
-      const int bytes = (int)p.bytes[t];
-      const long long first = group * kCopyGroup;
-      const int pairs = (int)min((long long)kCopyGroup, n - first);
-      const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
-      if ((at & 15) == 0)
-        copy_group<uint4>(p, p.base[t], bytes, first, pairs);
-      else if ((at & 3) == 0)
-        copy_group<uint32_t>(p, p.base[t], bytes, first, pairs);
-      else
-        copy_group<uint8_t>(p, p.base[t], bytes, first, pairs);
-    }
+  // units: a pair of a tensor with large blocks, then a group of pairs of one with
+  // small blocks. The next unit's pair is loaded while this one's bytes move.
+  const long long many = n * p.large;
+  auto pair_of = [&](long long u) -> long long { return u <= 0xffffffffLL ? (unsigned)u / (unsigned)p.large : u / p.large; };
+  long long u = blockIdx.x;
+  CopyPair next{-1, -1};
+  if (u < many) next = copy_pair(p, pair_of(u));
+  for (; u < many; u += gridDim.x) {
+    const CopyPair c = next;
+    const int t = (int)(u - pair_of(u) * p.large);
+    if (u + gridDim.x < many) next = copy_pair(p, pair_of(u + gridDim.x));
+    if (!copy_counts(p, c)) continue;
+    const long long bytes = p.bytes[t];
+    const char* s = p.base[t] + c.src * bytes;
+    char* d = p.base[t] + c.dst * bytes;
+    const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
+    if ((at & 15) == 0)
+      copy_words<uint4>(d, s, bytes);
+    else if ((at & 3) == 0)
+      copy_words<uint32_t>(d, s, bytes);
+    else
+      copy_words<uint8_t>(d, s, bytes);
+  }
+  for (; u < many + groups * small; u += gridDim.x) {
+    const long long group = (u - many) / small;
+    const int t = p.large + (int)(u - many - group * small);
+    const int bytes = (int)p.bytes[t];
+    const long long first = group * kCopyGroup;
+    const int pairs = (int)min((long long)kCopyGroup, n - first);
+    const unsigned long long at = (unsigned long long)p.base[t] | (unsigned long long)bytes;
+    if ((at & 15) == 0)
+      copy_group<uint4>(p, p.base[t], bytes, first, pairs);
+    else if ((at & 3) == 0)
+      copy_group<uint32_t>(p, p.base[t], bytes, first, pairs);
+    else
+      copy_group<uint8_t>(p, p.base[t], bytes, first, pairs);
   }
 }
 
@@ -144,18 +158,19 @@ struct CompactParams {
   int* status;
 };
 
-// The block of entry (i, pg) when its page holds a token that counts, else -1.
-__device__ __forceinline__ int compact_live(const CompactParams& p, int i, int pg, bool flag, bool* live) {
+// The block of entry e of the table when its page holds a token that counts,
+// else -1. (The length and the entry are loaded side by side.)
+__device__ __forceinline__ int compact_live(const CompactParams& p, long long e, bool flag) {
+  const int b = __ldg(p.page_table + e);
+  const int i = (int)(e <= 0xffffffffLL ? (unsigned)e / (unsigned)p.width : e / p.width);
+  const long long at = (e - (long long)i * p.width) * p.page;
   long long L = __ldg(p.lens + i);
   const long long cap = (long long)p.width * p.page;
   if (L > cap) {
     if (flag && p.status) atomicOr(p.status, CA_STATUS_LENS);
     L = cap;
   }
-  const long long at = (long long)pg * p.page;
-  *live = at < L && (p.left < 0 || at + p.page > L - 1 - p.left || at < p.sinks);
-  if (!*live) return -1;
-  const int b = __ldg(p.page_table + (long long)i * p.width + pg);
+  if (at >= L || !(p.left < 0 || at + p.page > L - 1 - p.left || at < p.sinks)) return -1;
   if (b < 0 || b >= p.num_blocks) {
     if (flag && p.status) atomicOr(p.status, CA_STATUS_TABLE);
     return -1;
@@ -188,10 +203,15 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
   for (int x = threadIdx.x; x < words; x += kPlanThreads) plan_bits[x] = 0u;
   __syncthreads();
   const long long entries = (long long)p.B * p.width;
-  for (long long e = threadIdx.x; e < entries; e += kPlanThreads) {
-    const int i = (int)(e / p.width);
-    bool live;
-    const int b = compact_live(p, i, (int)(e - (long long)i * p.width), true, &live);
+  int held[kPlanHeld];
+#pragma unroll
+  for (int k = 0; k < kPlanHeld; ++k) {
+    const long long e = threadIdx.x + k * kPlanThreads;
+    held[k] = e < entries ? compact_live(p, e, true) : -1;
+    if (held[k] >= 0) atomicOr(plan_bits + (held[k] >> 5), 1u << (held[k] & 31));
+  }
+  for (long long e = threadIdx.x + kPlanHeld * kPlanThreads; e < entries; e += kPlanThreads) {
+    const int b = compact_live(p, e, true);
     if (b >= 0) atomicOr(plan_bits + (b >> 5), 1u << (b & 31));
   }
   __syncthreads();
@@ -225,13 +245,15 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
   __syncthreads();  // (the CTA's writes of moves are visible to it)
   for (int k = threadIdx.x; k < count; k += kPlanThreads) p.place[p.moves[2 * k]] = p.moves[2 * k + 1];
   __syncthreads();
-  for (long long e = threadIdx.x; e < entries; e += kPlanThreads) {
-    const int i = (int)(e / p.width);
-    bool live;
-    const int b = compact_live(p, i, (int)(e - (long long)i * p.width), false, &live);
-    // an entry no row can use becomes -1, and so does a bad one (flagged above)
-    p.new_table[e] = b < 0 ? -1 : (b >= n ? p.place[b] : b);
+  // an entry no row can use becomes -1, and so does a bad one (flagged above)
+  auto placed = [&](int b) { return b < 0 ? -1 : (b >= n ? p.place[b] : b); };
+#pragma unroll
+  for (int k = 0; k < kPlanHeld; ++k) {
+    const long long e = threadIdx.x + k * kPlanThreads;
+    if (e < entries) p.new_table[e] = placed(held[k]);
   }
+  for (long long e = threadIdx.x + kPlanHeld * kPlanThreads; e < entries; e += kPlanThreads)
+    p.new_table[e] = placed(compact_live(p, e, false));
 }
 
 }  // namespace ca
