@@ -33,7 +33,9 @@ cudaError_t launch(SplitParams prm, int ctas, bool after_append, int device, cud
   cfg.numAttrs = after_append ? 1 : 0;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
   if (e != cudaSuccess) return e;
-  cfg.blockDim = dim3(32 * kSplitMergeShares * (E / 16));
+  // few items: each is cut into many pieces, which more warps join side by side
+  const int shares = 8LL * prm.B * prm.IH <= ctas ? kSplitMergeShares : kSplitMergeShares / 2;
+  cfg.blockDim = dim3(32 * shares * (E / 16));
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, split_merge_kernel<KIND, QT, E>, prm);

@@ -80,10 +80,11 @@ constexpr int kSplitAhead = 2;        // tiles ahead whose lines are brought to 
 // may pass by kSlack before it moves (a vote per tile, no reduction): up to 2^14
 // for f16, whose smallest step is then 2^-30 of the reference's weight.
 constexpr float kUp = 6.f, kSlack = 8.f;
-// Shares of an item's pieces that a join takes side by side. 2 (blocks of 512
-// threads, all resident at once) against 4: 32.5 and 35 us with two or three
-// pieces an item (32 x 16 heads), 57 and 55 us with 37 (one long sequence).
-constexpr int kSplitMergeShares = 2;
+// Shares of an item's pieces that a join takes side by side: this many when items
+// are few and cut into many pieces (one long sequence, 37 pieces: 57 -> 56 us),
+// else half (blocks of 512 threads, all resident at once: two or three pieces an
+// item, 32 x 16 heads, 35 -> 33 us).
+constexpr int kSplitMergeShares = 4;  // at most
 
 struct SplitParams {
   const void* q;
@@ -1216,12 +1217,13 @@ __global__ void __launch_bounds__(32 * kSplitMergeShares * (E / 16))
   __shared__ float shares[kSplitMergeShares * C::kPieceFloats];
   const int lane = threadIdx.x & 31;
   const int j = (threadIdx.x >> 5) % C::NM, share = (threadIdx.x >> 5) / C::NM;
+  const int count = (int)blockDim.x / (32 * C::NM);  // shares
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
   const int* m = p.meta + 4 * c;
   if (m[3] != 1) return;
   const int n = m[2] - c + 1;
-  const int per = (n + kSplitMergeShares - 1) / kSplitMergeShares;
+  const int per = (n + count - 1) / count;
   const int k0 = share * per, k1 = min(n, k0 + per);
   // one group of four registers, and (m, l) with it
   SplitState<1> st;
@@ -1263,7 +1265,7 @@ __global__ void __launch_bounds__(32 * kSplitMergeShares * (E / 16))
     SplitState<C::NM> all;
     all.clear();
 #pragma unroll 1
-    for (int r = 0; r < kSplitMergeShares; ++r) all.join(shares + r * C::kPieceFloats, lane);
+    for (int r = 0; r < count; ++r) all.join(shares + r * C::kPieceFloats, lane);
     split_write<KIND, QT, E>(p, all, m[0], m[1], lane);
   }
 }
