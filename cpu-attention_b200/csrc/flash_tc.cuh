@@ -18,7 +18,8 @@
 //              in the order S_A S_B | PV_A(j) S_A(j+1) | PV_B(j) S_B(j+1) ...,
 //              so the tensor core works on one tile while the other tile's
 //              softmax runs (ping-pong).
-//   warps 2-3  idle (their registers go to the softmax warpgroups)
+//   warps 2-3  idle (their registers go to the softmax warpgroups); windowed and
+//              packed, they clear the rows of V behind a sequence's end
 //   warps 4-7  softmax of tile A, warps 8-11 of tile B: thread = query row =
 //              TMEM lane. The S row comes into registers in one TMEM round
 //              trip, the row max is taken, bf16 P is written back over the S
@@ -79,7 +80,7 @@ struct TcCfg {
 };
 
 struct TcBars {
-  uint64_t q, kf[4], ke[4], vf[4], ve[4], s[2], p[2], pv[2], fin;
+  uint64_t q, kf[4], ke[4], vf[4], ve[4], s[2], p[2], pv[2], fin, past, cleared;
   uint32_t tmem;
   int abort;
 };
@@ -226,6 +227,10 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
     return j;
   };
   const int nt = max(nt0, nt1);
+  // Packed: rows of the last tile from `own` on are another sequence's or padding.
+  // Their weights are 0, but 0 times an infinity or NaN of theirs is not: warps
+  // 2-3 clear them in V once the tile is there, while its softmax runs.
+  const int own = WIN && a.cu_k && nt > 0 ? min(C::BN, max(0, Lk - tiles.real(nt - 1) * C::BN)) : C::BN;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q, 1);
@@ -241,6 +246,8 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       mbar_init(&bars->pv[s], 1);
     }
     mbar_init(&bars->fin, 1);
+    mbar_init(&bars->past, 1);
+    mbar_init(&bars->cleared, 64);
     bars->abort = 0;
     fence_barrier_init();
   }
@@ -306,6 +313,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       constexpr uint32_t idS = tc::idesc_bf16(128, 128, 0);
       constexpr uint32_t idO = tc::idesc_bf16(128, E, 1);
       bool ok = tc_wait(&bars->q, 0, abort, a.status);
+      bool cleared = false;  // (asked for)
       tc::fence_after_sync();
       // S_x(j) = Q_x K_j^T; the last user of K_j releases its slot
       auto issue_s = [&](int x, int j) -> bool {
@@ -326,8 +334,15 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       // O_x += P_x(j) V_j; the last user of V_j releases its slot
       auto issue_pv = [&](int x, int j) -> bool {
         const int vs = j % C::VST;
+        const bool clear = WIN && own < C::BN && j == nt - 1;
+        if (clear && !cleared) {
+          if (!tc_wait(&bars->vf[vs], (j / C::VST) & 1, abort, a.status)) return false;
+          mbar_arrive(&bars->past);
+          cleared = true;
+        }
         if (!tc_wait(&bars->p[x], seq(x, j) & 1, abort, a.status)) return false;
         if (!tc_wait(&bars->vf[vs], (j / C::VST) & 1, abort, a.status)) return false;
+        if (clear && !tc_wait(&bars->cleared, 0, abort, a.status)) return false;
         tc::fence_after_sync();
         const uint32_t vaddr = smem_u32(sV + vs * C::TILE_BYTES);
 #pragma unroll
@@ -353,6 +368,17 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       // every MMA this thread issued has retired before TMEM is released
       tc::commit(&bars->fin);
       mbar_wait_bounded(&bars->fin, 0, kWaitLimitNs);
+    }
+  } else if (WIN && warp < 4) {
+    // ---------------------------------------- rows of V past the sequence's end
+    if (own < C::BN && tc_wait(&bars->past, 0, abort, a.status)) {
+      uint8_t* v = sV + ((nt - 1) % C::VST) * C::TILE_BYTES;  // (the swizzle stays inside a row)
+#pragma unroll
+      for (int ch = 0; ch < C::NCH; ++ch)
+        for (int at = own * C::SWB + ((int)threadIdx.x - 64) * 16; at < C::CH_BYTES; at += 64 * 16)
+          *reinterpret_cast<uint4*>(v + ch * C::CH_BYTES + at) = make_uint4(0u, 0u, 0u, 0u);
+      fence_proxy_async_smem();  // the tensor core reads them
+      mbar_arrive(&bars->cleared);
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax

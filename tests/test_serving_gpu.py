@@ -556,6 +556,31 @@ def test_prefill_window_packed(dtype, left, right, sinks):
                 assert torch.equal(out[a:z], dense[0]) and torch.equal(lse[:, a:z], dl[0])
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("causal,left,right,sinks", [(True, 40, 0, 4), (False, 130, 20, 0), (False, -1, 300, 1)])
+def test_prefill_window_packed_rows_of_others(dtype, hd, causal, left, right, sinks):
+    """What another sequence's rows, or padding behind the last one, hold (NaN, infinities) reaches no output."""
+    C = api()
+    lens, pad = [5, 130, 1, 300, 128, 77], 60
+    g = torch.Generator().manual_seed(hd)
+    t = sum(lens) + pad
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    q, k, v = (torch.randn(t, n, hd, generator=g).to(dtype).to(DEV) for n in (4, 2, 2))
+    opts = dict(causal=causal, window_size=(left, right), sink_tokens=sinks, return_attn_probs=True)
+    want, want_lse = C.flash_attn_varlen_func(q, k, v, cu, cu, 300, 300, **opts)
+    for bad in (1, 3, 5):  # the even sequences and the padding; the padding alone
+        kept = torch.zeros(t, dtype=torch.bool, device=DEV)
+        for i, n in enumerate(lens):
+            if i % 2 or bad == 5:
+                kept[int(cu[i]):int(cu[i + 1])] = True
+        kk, vv = k.clone(), v.clone()
+        kk[~kept] = math.nan
+        vv[~kept] = (math.nan, math.inf, -math.inf)[bad // 2]
+        out, lse = C.flash_attn_varlen_func(q, kk, vv, cu, cu, 300, 300, **opts)
+        assert torch.equal(out[kept], want[kept]) and torch.equal(lse[:, kept], want_lse[:, kept])
+
+
 def test_prefill_window_that_hides_nothing():
     """A window as long as the sequences gives the result of no window (fp32: the same tiles, the same bits)."""
     g = torch.Generator().manual_seed(0)
