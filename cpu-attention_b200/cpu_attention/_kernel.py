@@ -62,6 +62,8 @@ SIGNATURES = {
     "ca_compact_workspace_bytes": (_SZ, [_I64]),
     "ca_compact_blocks": (_I32, [_P, _PI64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ, _P,
                                  _P]),
+    "ca_compact_blocks_ex": (_I32, [_P, _PI64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ,
+                                    _P, _P]),
     "ca_status": (_I32, [_P, _I32, _P]),
     "ca_set_wait_limit_ns": (None, [ctypes.c_uint64]),
     "ca_last_cuda_error": (ctypes.c_char_p, []),

@@ -431,15 +431,18 @@ def copy_blocks(rt, caches, pairs):
     return _checked(dev, True) if _check_rc(rc) else None
 
 
-def compact_blocks(rt, caches, page_table, lens, page, left, sinks):
+def compact_blocks(rt, caches, page_table, lens, page, left, sinks, reserved=None):
     """The blocks in use moved to the front of every tensor ``[blocks, ...]``:
-    (the renumbered table, how many are in use as int32 ``[1]``), or None."""
+    (the renumbered table, how many are in use as int32 ``[1]``), or None.
+    ``reserved`` (int32 ``[seqs]``): the lengths up to which pages are kept."""
     del rt
     fast = K.fastpath()
-    if fast is not None and _plain_tensors(page_table, lens, *caches):
-        return _checked(page_table.device, fast.compact_blocks(caches, page_table, lens, page, left, sinks))
-    dev = _cuda(page_table, lens, *caches)
+    if fast is not None and _plain_tensors(page_table, lens, *caches) and _plain_or_none(reserved):
+        return _checked(page_table.device, fast.compact_blocks(caches, page_table, lens, page, left, sinks, reserved))
+    dev = _cuda(page_table, lens, reserved, *caches)
     if dev is None or not caches or page_table.dim() != 2 or not _table_ok(page_table, page_table.shape[0]):
+        return None
+    if reserved is not None and not _int_vector(reserved, torch.int32, page_table.shape[0]):
         return None
     got = _block_tensors(caches, dev) if _int_vector(lens, torch.int32, page_table.shape[0]) else None
     if got is None:
@@ -451,8 +454,8 @@ def compact_blocks(rt, caches, page_table, lens, page, left, sinks):
     need = int(K.library().ca_compact_workspace_bytes(blocks))
     scratch = torch.empty(need, dtype=torch.uint8, device=dev)
     with K.on_device(dev):
-        rc = K.library().ca_compact_blocks(base, sizes, count, blocks, page_table.data_ptr(), lens.data_ptr(),
-                                           page_table.shape[0], page_table.shape[1], page, left, sinks,
-                                           table.data_ptr(), used.data_ptr(), scratch.data_ptr(), need,
-                                           ws.data_ptr(), stream)
+        rc = K.library().ca_compact_blocks_ex(base, sizes, count, blocks, page_table.data_ptr(), lens.data_ptr(),
+                                              _ptr(reserved), page_table.shape[0], page_table.shape[1], page, left,
+                                              sinks, table.data_ptr(), used.data_ptr(), scratch.data_ptr(), need,
+                                              ws.data_ptr(), stream)
     return _checked(dev, (table, used)) if _check_rc(rc) else None

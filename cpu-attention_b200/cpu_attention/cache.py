@@ -235,15 +235,21 @@ def copy_blocks(caches, block_mapping) -> None:
         raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
 
 
-def compact_blocks(caches, page_table, cache_seqlens, page_block_size, window_size=(-1, -1), sink_tokens=0):
+def compact_blocks(caches, page_table, cache_seqlens, page_block_size, window_size=(-1, -1), sink_tokens=0,
+                   reserved_seqlens=None):
     """Moves the blocks in use to the front of the pool.
 
     In use are the blocks behind ``page_table`` (int32 ``[batch, max_blocks]``)
-    whose page holds one of its sequence's ``cache_seqlens`` tokens -- give the
-    reserved lengths to keep pages for tokens to come -- and, with a window
-    (``window_size``, ``sink_tokens`` as in ``flash_attn_with_kvcache``), is not
-    wholly between the first tokens and the window: those pages are freed. With
-    n blocks in use, each one with an id of n or more moves, in ascending order,
+    whose page holds one of its sequence's ``cache_seqlens`` tokens and, with a
+    window (``window_size``, ``sink_tokens`` as in ``flash_attn_with_kvcache``),
+    is not wholly between the first tokens and the window: those pages are
+    freed. ``cache_seqlens`` counts every token in the cache; tokens that a
+    decode has just appended are not in the lengths it was given. To keep pages
+    for tokens to come, give the lengths they will reach as ``reserved_seqlens``
+    (int32 ``[batch]``; below ``cache_seqlens`` it changes nothing): the window
+    is measured from ``cache_seqlens`` all the same, so nothing that is still
+    seen is freed. A negative ``cache_seqlens`` leaves a sequence out. With n
+    blocks in use, each one with an id of n or more moves, in ascending order,
     to the free ids below n, in every tensor of ``caches`` (contiguous
     ``[num_blocks, ...]``); blocks that sequences share move once and stay
     shared.
@@ -269,10 +275,16 @@ def compact_blocks(caches, page_table, cache_seqlens, page_block_size, window_si
         raise ValueError("cpu_attention: page_table must be int32 [batch, max_blocks]")
     if lens.dtype != torch.int32 or tuple(lens.shape) != (table.shape[0],):
         raise ValueError("cpu_attention: cache_seqlens must be an int32 [batch] tensor")
+    if reserved_seqlens is not None:
+        (reserved_seqlens,) = _plain(reserved_seqlens)
+        if not isinstance(reserved_seqlens, torch.Tensor) or reserved_seqlens.dtype != torch.int32 \
+                or tuple(reserved_seqlens.shape) != (table.shape[0],):
+            raise ValueError("cpu_attention: reserved_seqlens must be an int32 [batch] tensor")
     dev = caches[0].device
     if dev.type != "cuda" or any(t.device != dev for t in caches):
         raise ValueError(f"cpu_attention: the caches must be CUDA tensors on one device (the first is on {dev})")
-    got = _native.compact_blocks(0, caches, table.contiguous().to(dev), lens.contiguous().to(dev), page, left, sinks)
+    table, lens, reserved = (x if x is None else x.contiguous().to(dev) for x in (table, lens, reserved_seqlens))
+    got = _native.compact_blocks(0, caches, table, lens, page, left, sinks, reserved)
     if got is None:
         raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
     return got

@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const __grid_
 struct CompactParams {
   const int* page_table;  // [B, width]
   const int* lens;
+  const int* reserved;  // [B] lengths up to which pages are kept (at least lens), or NULL
   int* new_table;  // [B, width]
   int* used;       // [1]
   int* moves;      // [num_blocks][2]: the first count[0] are set
@@ -158,19 +159,22 @@ struct CompactParams {
   int* status;
 };
 
-// The block of entry e of the table when its page holds a token that counts,
-// else -1. (The length and the entry are loaded side by side.)
+// The block of entry e of the table when its page holds a token that counts or
+// is reserved for one to come, else -1. The window ends at the tokens that are
+// there, whatever is reserved. (The length and the entry are loaded side by side.)
 __device__ __forceinline__ int compact_live(const CompactParams& p, long long e, bool flag) {
   const int b = __ldg(p.page_table + e);
   const int i = (int)(e <= 0xffffffffLL ? (unsigned)e / (unsigned)p.width : e / p.width);
   const long long at = (e - (long long)i * p.width) * p.page;
   long long L = __ldg(p.lens + i);
   const long long cap = (long long)p.width * p.page;
-  if (L > cap) {
+  long long end = p.reserved && L >= 0 ? max(L, (long long)__ldg(p.reserved + i)) : L;
+  if (end > cap) {
     if (flag && p.status) atomicOr(p.status, CA_STATUS_LENS);
-    L = cap;
+    end = cap;
+    L = min(L, cap);
   }
-  if (at >= L || !(p.left < 0 || at + p.page > L - 1 - p.left || at < p.sinks)) return -1;
+  if (at >= end || !(p.left < 0 || at + p.page > L - 1 - p.left || at < p.sinks)) return -1;
   if (b < 0 || b >= p.num_blocks) {
     if (flag && p.status) atomicOr(p.status, CA_STATUS_TABLE);
     return -1;

@@ -252,6 +252,16 @@ int ca_compact_blocks(void* const* base, const int64_t* block_bytes, int64_t ten
                       const int32_t* page_table, const int32_t* lens, int64_t batch, int64_t table_width,
                       int64_t page, int64_t window_left, int64_t sink_tokens, int32_t* new_table, int32_t* used,
                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return ca_compact_blocks_ex(base, block_bytes, tensors, num_blocks, page_table, lens, nullptr, batch, table_width,
+                              page, window_left, sink_tokens, new_table, used, workspace, workspace_bytes, status,
+                              stream);
+}
+
+int ca_compact_blocks_ex(void* const* base, const int64_t* block_bytes, int64_t tensors, int64_t num_blocks,
+                         const int32_t* page_table, const int32_t* lens, const int32_t* reserved, int64_t batch,
+                         int64_t table_width, int64_t page, int64_t window_left, int64_t sink_tokens,
+                         int32_t* new_table, int32_t* used, void* workspace, size_t workspace_bytes, int32_t* status,
+                         void* stream) {
   int rc = copy_checks(base, block_bytes, tensors, num_blocks);
   if (rc) return rc;
   if (!page_ok(page)) return CA_EPAGE;
@@ -264,6 +274,7 @@ int ca_compact_blocks(void* const* base, const int64_t* block_bytes, int64_t ten
   ca::CompactParams p{};
   p.page_table = page_table;
   p.lens = lens;
+  p.reserved = reserved;
   p.new_table = new_table;
   p.used = used;
   p.count = static_cast<int*>(workspace);

@@ -424,11 +424,13 @@ py::object copy_blocks(const std::vector<at::Tensor>& caches, const at::Tensor& 
 }
 
 py::object compact_blocks(const std::vector<at::Tensor>& caches, const at::Tensor& pt, const at::Tensor& lens,
-                          int64_t page, int64_t left, int64_t sinks) {
+                          int64_t page, int64_t left, int64_t sinks, const c10::optional<at::Tensor>& reserved) {
   if (!pt.is_cuda() || caches.empty()) return py::none();
   const auto device = pt.device();
   if (pt.dim() != 2 || pt.scalar_type() != at::kInt || !pt.is_contiguous() || !lens.is_cuda() ||
       lens.device() != device || !int_vector(lens, at::kInt, pt.size(0)))
+    return py::none();
+  if (reserved && (!reserved->is_cuda() || reserved->device() != device || !int_vector(*reserved, at::kInt, pt.size(0))))
     return py::none();
   std::vector<void*> base;
   std::vector<int64_t> bytes;
@@ -441,10 +443,11 @@ py::object compact_blocks(const std::vector<at::Tensor>& caches, const at::Tenso
   at::Tensor table = at::empty(pt.sizes(), pt.options()), used = at::empty({1}, pt.options());
   const size_t need = ca_compact_workspace_bytes(blocks);
   at::Tensor scratch = at::empty({(int64_t)need}, pt.options().dtype(at::kByte));
-  const int rc = ca_compact_blocks(base.data(), bytes.data(), (int64_t)base.size(), blocks, pt.data_ptr<int32_t>(),
-                                   lens.data_ptr<int32_t>(), pt.size(0), pt.size(1), page, left, sinks,
-                                   table.data_ptr<int32_t>(), used.data_ptr<int32_t>(), scratch.data_ptr(), need,
-                                   static_cast<int32_t*>(ws.data_ptr()), stream);
+  const int rc = ca_compact_blocks_ex(
+      base.data(), bytes.data(), (int64_t)base.size(), blocks, pt.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+      reserved ? reserved->data_ptr<int32_t>() : nullptr, pt.size(0), pt.size(1), page, left, sinks,
+      table.data_ptr<int32_t>(), used.data_ptr<int32_t>(), scratch.data_ptr(), need,
+      static_cast<int32_t*>(ws.data_ptr()), stream);
   if (rc == CA_ECUDA) throw std::runtime_error(std::string("cpu_attention: ") + ca_last_cuda_error());
   if (rc != CA_OK) return py::none();
   return py::make_tuple(table, used);
@@ -472,7 +475,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("sinks"), py::arg("lse"), py::arg("cu_q"), py::arg("cu_k"), py::arg("max_q"), py::arg("max_k"));
   m.def("copy_blocks", &copy_blocks, "block copies; True, or None when declined", py::arg("caches"), py::arg("pairs"));
   m.def("compact_blocks", &compact_blocks, "pack the blocks in use; (table, used), or None when declined",
-        py::arg("caches"), py::arg("page_table"), py::arg("lens"), py::arg("page"), py::arg("left"), py::arg("sinks"));
+        py::arg("caches"), py::arg("page_table"), py::arg("lens"), py::arg("page"), py::arg("left"), py::arg("sinks"),
+        py::arg("reserved") = py::none());
   m.def("workspace", &py_workspace, "the workspace tensor of (device, stream), at least nbytes long",
         py::arg("device"), py::arg("stream"), py::arg("nbytes"));
 }

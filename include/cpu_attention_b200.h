@@ -311,7 +311,12 @@ CA_API int ca_decode_split(const void* q, int64_t q_stride, void* k_cache,
  * ca_compact_blocks: packs the blocks in use. In use are the blocks of the
  * table entries whose page starts below lens[i] and, with window_left >= 0, is
  * not wholly between the first sink_tokens tokens and the window of a query at
- * lens[i] - 1. With n of them, the k-th smallest id >= n in use moves to the
+ * lens[i] - 1. lens counts every token that is in the cache: what a decode has
+ * appended, too (it leaves its `lens`, the lengths before, as they are).
+ * ca_compact_blocks_ex takes `reserved` beside it (int32 [batch], or NULL):
+ * pages that start below reserved[i] are kept for tokens to come, while the
+ * window stays the one at lens[i] - 1; a value below lens[i] counts as lens[i],
+ * and lens[i] < 0 leaves sequence i without blocks. With n of them, the k-th smallest id >= n in use moves to the
  * k-th smallest free id < n, in every tensor. new_table gets the renumbered
  * table, -1 in entries not in use (bad entries in use, flagged
  * CA_STATUS_TABLE, too); used[0] = n. page_table is left as it was. workspace:
@@ -330,6 +335,14 @@ CA_API int ca_compact_blocks(void* const* base, const int64_t* block_bytes,
              int64_t page, int64_t window_left, int64_t sink_tokens,
              int32_t* new_table, int32_t* used, void* workspace,
              size_t workspace_bytes, int32_t* status, void* stream);
+
+CA_API int ca_compact_blocks_ex(void* const* base, const int64_t* block_bytes,
+             int64_t tensors, int64_t num_blocks, const int32_t* page_table,
+             const int32_t* lens, const int32_t* reserved, int64_t batch,
+             int64_t table_width, int64_t page, int64_t window_left,
+             int64_t sink_tokens, int32_t* new_table, int32_t* used,
+             void* workspace, size_t workspace_bytes, int32_t* status,
+             void* stream);
 
 /* ---- runtime ------------------------------------------------------------ */
 /* The status word of a decode workspace (ORed CA_STATUS_* bits since the last

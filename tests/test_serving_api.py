@@ -245,3 +245,12 @@ def test_layouts_round_trip():
     packed = S.pack(x.bfloat16(), True, "f")[1, 2].flatten()
     perm = torch.from_numpy(paged.k_perm(16, 32, True))
     assert torch.equal(packed[perm], x.bfloat16()[1, 2])
+
+
+def test_compact_reserved_lengths_refusals():
+    caches, bt, lens = [torch.zeros(4, 3)], torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for reserved in (lens.long(), torch.zeros(2, dtype=torch.int32), lens.view(1, 1), 5, [5]):
+        with pytest.raises(ValueError, match="reserved_seqlens"):
+            C.compact_blocks(caches, bt, lens, 16, reserved_seqlens=reserved)
+    with pytest.raises(ValueError, match="CUDA"):
+        C.compact_blocks(caches, bt, lens, 16, reserved_seqlens=lens)

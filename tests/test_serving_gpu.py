@@ -765,3 +765,53 @@ def test_serving_run(kind):
                 err = (out[x, 0, a * 4:(a + 1) * 4].double().cpu() - ref).abs()
                 assert (err <= tol).all(), (step, i, err.max().item())
     assert status() == 0
+
+
+@pytest.mark.parametrize("kind", ["8bit", "bf16", "fp32"])
+@pytest.mark.parametrize("left,sinks", [(63, 0), (30, 20), (-1, 0)])
+def test_compact_keeps_what_is_seen_and_reserved(kind, left, sinks):
+    """Lengths reserved ahead keep their pages; the window stays the one of the tokens that are there, so the next
+    decode answers as if nothing had moved."""
+    C = api()
+    h, hk, d, page, ahead = 4, 2, 64, 16, 64
+    dtype = FP32 if kind == "fp32" else BF16
+    lens = [100, 3, 0, 256, 31, -1]
+    pc = S.Paged(kind, lens, hk, d, page, dtype, seed=left + 71, room=ahead)
+    pc.left, pc.sinks = left, sinks
+    caches = [t for t in (pc.k_cache, pc.v_cache, pc.k_scale, pc.v_scale) if t is not None]
+    reserved = [n + ahead for n in lens[:4]] + [2, ahead]  # (below the length: the length counts)
+    q = torch.randn(len(lens), 1, h, d, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    opts = dict(window_size=(left, 0), sink_tokens=sinks)
+    want = C.flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt, **pc.opts(), **opts)
+    S.check_decode(want, None, q, pc, h)
+    old = pc.bt.tolist()
+    keep = [[n >= 0 and p * page < max(n, r) and (left < 0 or (p + 1) * page > n - 1 - left or p * page < sinks)
+             for p in range(len(row))] for row, n, r in zip(old, lens, reserved)]
+    used_ids = {b for row, on in zip(old, keep) for b, x in zip(row, on) if x}
+    free = [b for b in range(len(used_ids)) if b not in used_ids]
+    moves = dict(zip(sorted(b for b in used_ids if b >= len(used_ids)), free))
+    reserved = torch.tensor(reserved, dtype=torch.int32)
+    for where in (DEV, "cpu"):  # the second call finds everything packed
+        table, used = C.compact_blocks(caches, pc.bt, pc.L, page, reserved_seqlens=reserved.to(where), **opts)
+        if where == DEV:
+            assert table.tolist() == [[moves.get(b, b) if x else -1 for b, x in zip(row, on)]
+                                      for row, on in zip(old, keep)]
+            first = table
+        else:
+            assert torch.equal(table, first)
+        assert used.tolist() == [len(used_ids)]
+        pc.bt = table
+        got = C.flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=table, **pc.opts(),
+                                        **opts)
+        assert torch.equal(got, want)
+    assert status() == 0
+    # the ctypes path answers the same
+    from cpu_attention import _kernel as K, _native
+    fast, K._FAST = K.fastpath(), False
+    try:
+        again, n = _native.compact_blocks(0, caches, pc.bt, pc.L, page, left, sinks, reserved.to(DEV))
+    finally:
+        K._FAST = fast
+    assert torch.equal(again, first) and n.tolist() == used.tolist()
+    C.compact_blocks(caches, pc.bt, pc.L, page, reserved_seqlens=reserved.to(DEV) + 10000, **opts)
+    assert status() & kernel().STATUS_LENS
