@@ -254,3 +254,33 @@ def test_compact_reserved_lengths_refusals():
             C.compact_blocks(caches, bt, lens, 16, reserved_seqlens=reserved)
     with pytest.raises(ValueError, match="CUDA"):
         C.compact_blocks(caches, bt, lens, 16, reserved_seqlens=lens)
+
+
+def step_example():
+    """The decode step with compaction that INTEGRATION.md shows, as code."""
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    blocks = re.findall(r"```python\n(.*?)```", open(os.path.join(root, "INTEGRATION.md")).read(), re.S)
+    (code,) = [b for b in blocks if "compact_blocks" in b]
+    return code
+
+
+def test_step_example_packs_with_the_new_token_counted(monkeypatch):
+    """The decode leaves its lengths as they were; the compaction behind it has to count the token it appended."""
+    lens, seen = torch.tensor([16, 5], dtype=torch.int32), {}
+
+    def attend(*args, cache_seqlens, **kwargs):
+        seen["attend"] = cache_seqlens.clone()
+        return args[0]
+
+    def pack(caches, table, cache_seqlens, page, **kwargs):
+        seen["pack"] = cache_seqlens.clone()
+        return table, torch.zeros(1, dtype=torch.int32)
+
+    monkeypatch.setattr(C, "flash_attn_with_kvcache", attend)
+    monkeypatch.setattr(C, "compact_blocks", pack)
+    names = dict.fromkeys("q k v k_cache v_cache k_scale v_scale table".split())
+    exec(step_example(), dict(names, lens=lens, page=16))
+    assert seen["attend"].tolist() == [16, 5] and seen["pack"].tolist() == [17, 6]

@@ -815,3 +815,31 @@ def test_compact_keeps_what_is_seen_and_reserved(kind, left, sinks):
     assert torch.equal(again, first) and n.tolist() == used.tolist()
     C.compact_blocks(caches, pc.bt, pc.L, page, reserved_seqlens=reserved.to(DEV) + 10000, **opts)
     assert status() & kernel().STATUS_LENS
+
+
+def test_step_example_keeps_the_new_token():
+    """INTEGRATION.md's decode step with a compaction behind it, with lengths that end at a page: the next step finds
+    every token."""
+    from test_serving_api import step_example
+    C = api()
+    lens, page, width = [16, 32, 5, 0, 47], 16, 4
+    kc, vc, ks, vs = empty_8bit(40, 2, page, 64, 0)
+    g = torch.Generator().manual_seed(8)
+    table = torch.randperm(40, generator=g)[:5 * width].reshape(5, width).to(torch.int32).to(DEV)
+    hist = [torch.randn(5, 48, 2, 64, generator=g).bfloat16().to(DEV) for _ in range(2)]
+    names = dict(k_cache=kc, v_cache=vc, k_scale=ks, v_scale=vs, page=page, table=table)
+    for i, n in enumerate(lens):  # the tokens before
+        C.append_quantized(hist[0][i:i + 1, :n], hist[1][i:i + 1, :n], kc, vc, ks, vs,
+                           torch.zeros(1, dtype=torch.int32, device=DEV), table[i:i + 1])
+    before = [t.clone() for t in (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)]
+    L = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = torch.randn(5, 1, 4, 64, generator=g).bfloat16().to(DEV)
+    k, v = (torch.randn(5, 1, 2, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    exec(step_example(), names | dict(q=q, k=k, v=v, lens=L.clone()), names)
+    again = C.flash_attn_with_kvcache(q, kc, vc, cache_seqlens=L + 1, page_table=names["table"], k_descale=ks,
+                                      v_descale=vs, window_size=(4095, 0), sink_tokens=4)
+    assert torch.equal(again, names["out"])
+    want = C.flash_attn_with_kvcache(q, before[0].view(S.F8), before[1].view(S.F8), k=k, v=v, cache_seqlens=L,
+                                     page_table=table, k_descale=before[2], v_descale=before[3])
+    assert torch.equal(again, want) and status() == 0
+    assert int(names["used"]) == sum(-(-(n + 1) // page) for n in lens)
