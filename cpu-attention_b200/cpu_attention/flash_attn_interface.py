@@ -382,8 +382,8 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
     causal mask is bottom-right within each sequence. Returns ``[total_q,
     nheads, headdim]``, and with ``return_attn_probs`` also the float32
     ``[nheads, total_q]`` log-sum-exp. ``window_size`` and ``sink_tokens`` as in
-    ``flash_attn_func``, within each sequence; with a window, rows of other
-    sequences and behind the last one may hold anything.
+    ``flash_attn_func``, within each sequence. What rows of k/v of other
+    sequences and behind the last one hold reaches no output of a sequence.
     """
     window = _prefill_window(window_size, sink_tokens)
     lse = None

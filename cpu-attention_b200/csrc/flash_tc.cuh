@@ -18,8 +18,8 @@
 //              in the order S_A S_B | PV_A(j) S_A(j+1) | PV_B(j) S_B(j+1) ...,
 //              so the tensor core works on one tile while the other tile's
 //              softmax runs (ping-pong).
-//   warps 2-3  idle (their registers go to the softmax warpgroups); windowed and
-//              packed, they clear the rows of V behind a sequence's end
+//   warps 2-3  idle (their registers go to the softmax warpgroups); packed, they
+//              clear the rows of V behind a sequence's end
 //   warps 4-7  softmax of tile A, warps 8-11 of tile B: thread = query row =
 //              TMEM lane. The S row comes into registers in one TMEM round
 //              trip, the row max is taken, bf16 P is written back over the S
@@ -176,7 +176,10 @@ __device__ __forceinline__ uint32_t bit_range(int a, int b) {
   return below_b & ~below_a;
 }
 
-template <int E, bool CAUSAL, bool WIN>
+// PACKED: k/v may hold other sequences' rows behind this one's. (Its own
+// instantiation: dense launches, which have none, lost 3% at head_dim 128 to the
+// issuer's test for the tile to clear: 137.5 -> 141.7 us at 4096 tokens, 16 heads.)
+template <int E, bool CAUSAL, bool WIN, bool PACKED>
 __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant__ FlashTcArgs a) {
   using C = TcCfg<E>;
   extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
   // Packed: rows of the last tile from `own` on are another sequence's or padding.
   // Their weights are 0, but 0 times an infinity or NaN of theirs is not: warps
   // 2-3 clear them in V once the tile is there, while its softmax runs.
-  const int own = WIN && a.cu_k && nt > 0 ? min(C::BN, max(0, Lk - tiles.real(nt - 1) * C::BN)) : C::BN;
+  const int own = PACKED && a.cu_k && nt > 0 ? min(C::BN, max(0, Lk - (WIN ? tiles.real(nt - 1) : nt - 1) * C::BN)) : C::BN;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q, 1);
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       // O_x += P_x(j) V_j; the last user of V_j releases its slot
       auto issue_pv = [&](int x, int j) -> bool {
         const int vs = j % C::VST;
-        const bool clear = WIN && own < C::BN && j == nt - 1;
+        const bool clear = PACKED && own < C::BN && j == nt - 1;
         if (clear && !cleared) {
           if (!tc_wait(&bars->vf[vs], (j / C::VST) & 1, abort, a.status)) return false;
           mbar_arrive(&bars->past);
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(384, 1) flash_tc_kernel(const __grid_constant_
       tc::commit(&bars->fin);
       mbar_wait_bounded(&bars->fin, 0, kWaitLimitNs);
     }
-  } else if (WIN && warp < 4) {
+  } else if (PACKED && warp < 4) {
     // ---------------------------------------- rows of V past the sequence's end
     if (own < C::BN && tc_wait(&bars->past, 0, abort, a.status)) {
       uint8_t* v = sV + ((nt - 1) % C::VST) * C::TILE_BYTES;  // (the swizzle stays inside a row)
@@ -659,11 +662,14 @@ int flash_tc_launch(const FlashParams& p, int* status, cudaStream_t stream, std:
   a.right = p.right;
   a.sinks = p.sinks;
   a.status = status;
-  static unsigned char configured[3][64] = {};
-  static int regs_ok[3] = {0, 0, 0};  // 0: not checked, 1: as planned, -1: not
-  const int form = p.win ? 2 : (p.causal ? 1 : 0);
-  auto kern = p.win ? flash_tc_kernel<E, false, true>
-                    : (p.causal ? flash_tc_kernel<E, true, false> : flash_tc_kernel<E, false, false>);
+  static unsigned char configured[5][64] = {};
+  static int regs_ok[5] = {};  // 0: not checked, 1: as planned, -1: not
+  const int form = p.win ? 4 : (var ? 2 : 0) + (p.causal ? 1 : 0);
+  decltype(&flash_tc_kernel<E, false, false, false>) const kerns[5] = {
+      flash_tc_kernel<E, false, false, false>, flash_tc_kernel<E, true, false, false>,
+      flash_tc_kernel<E, false, false, true>, flash_tc_kernel<E, true, false, true>,
+      flash_tc_kernel<E, false, true, true>};  // (windowed, dense ones too)
+  auto kern = kerns[form];
   if (regs_ok[form] == 0) {
     // the register split assumes exactly REGS_LAUNCH registers per thread at
     // launch (a larger split would wait forever in setmaxnreg)

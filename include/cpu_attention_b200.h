@@ -215,7 +215,8 @@ CA_API int ca_flash(const void* q, const void* k, const void* v, void* out,
  *   [total_k, kv_heads, head_dim]; seq_q / seq_k are then the largest
  *   sequence lengths (no sequence may exceed them), the strides' batch entry
  *   is ignored, out is [total_q, heads, head_dim] and causal masks per
- *   sequence (bottom-right). total_q / total_k are ignored when dense.
+ *   sequence (bottom-right). total_q / total_k are ignored when dense. Rows of
+ *   k/v of other sequences, or behind the last one, may hold anything.
  */
 CA_API int ca_flash_ex(const void* q, const void* k, const void* v, void* out,
              float* lse, int64_t batch, int64_t seq_q, int64_t seq_k,

@@ -843,3 +843,34 @@ def test_step_example_keeps_the_new_token():
                                      page_table=table, k_descale=before[2], v_descale=before[3])
     assert torch.equal(again, want) and status() == 0
     assert int(names["used"]) == sum(-(-(n + 1) // page) for n in lens)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_packed_rows_of_others(dtype, hd, causal):
+    """Without a window too, what another sequence's rows, or padding behind the last one, hold (NaN, infinities)
+    reaches no output; queries and keys of different lengths, one sequence without keys."""
+    C = api()
+    lq, lk, pad = [5, 130, 1, 300, 128, 77, 3], [9, 130, 257, 300, 128, 40, 0], 60
+    g = torch.Generator().manual_seed(hd)
+    cq, ck = (torch.tensor([sum(n[:i]) for i in range(len(n) + 1)], dtype=torch.int32, device=DEV) for n in (lq, lk))
+    q = torch.randn(sum(lq), 4, hd, generator=g).to(dtype).to(DEV)
+    k, v = (torch.randn(sum(lk) + pad, 2, hd, generator=g).to(dtype).to(DEV) for _ in range(2))
+    call = lambda kk, vv: C.flash_attn_varlen_func(q, kk, vv, cq, ck, 300, 300, causal=causal,  # noqa: E731
+                                                   return_attn_probs=True)
+    want, want_lse = call(k, v)
+    assert torch.isfinite(want).all()
+    for bad in (math.nan, math.inf, -math.inf):
+        for keep in (0, 1, 2):  # the sequences of an even index, of an odd one, all of them
+            rows_q, rows_k = (torch.zeros(n, dtype=torch.bool, device=DEV) for n in (q.shape[0], k.shape[0]))
+            for i in range(len(lq)):
+                if keep == 2 or i % 2 == keep:
+                    rows_q[int(cq[i]):int(cq[i + 1])] = True
+                    rows_k[int(ck[i]):int(ck[i + 1])] = True
+            kk, vv = k.clone(), v.clone()
+            kk[~rows_k] = math.nan
+            vv[~rows_k] = bad
+            out, lse = call(kk, vv)
+            assert torch.equal(out[rows_q], want[rows_q]) and torch.equal(lse[:, rows_q], want_lse[:, rows_q])
+    assert status() == 0
