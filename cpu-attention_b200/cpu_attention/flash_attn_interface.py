@@ -121,8 +121,10 @@ def flash_attn_with_kvcache(
     caches: the query, at the last position, sees the last ``window_size[0] +
     1`` tokens and the first ``sink_tokens`` ones (``window_size[0] = -1``: all).
     Pages wholly between the two are never read; their page-table entries may
-    be anything (``compact_blocks`` frees them). Without ``sink_tokens`` a
-    window is refused, as in the reference.
+    be anything (``compact_blocks`` frees them), but for pages that get tokens
+    of ``k``/``v``: those are written wherever the entry names a block, and left
+    out in such a page where it is -1. Without ``sink_tokens`` a window is
+    refused, as in the reference.
     """
     # (every option at its default: the common case, decided without building
     # the option table -- an engine calls this once per layer and token)

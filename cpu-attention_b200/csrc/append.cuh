@@ -47,6 +47,7 @@ struct AppendParams {
   int n_new;         // tokens per sequence (dense), or the most of any (packed)
   int B, H, page;
   int pages;  // pages a sequence touches at most (packed: all of them)
+  long long left, sinks;  // the window of the decode behind this append (left < 0: none)
   int* status;
 };
 
@@ -66,14 +67,16 @@ __device__ __forceinline__ int append_tokens(const AppendParams& p, int i, long 
   return (int)(z - a);
 }
 
-// Entry b of page pg of sequence i, or -1 (flagged).
-__device__ __forceinline__ int append_block(const AppendParams& p, int i, long long pg, int b) {
+// Entry b of page pg, or -1: flagged, but where the page lies wholly between the
+// first tokens and the window that sees `len` tokens (it may be freed already).
+__device__ __forceinline__ int append_block(const AppendParams& p, long long pg, int b, long long len) {
   if (pg >= p.pt_stride) {
     if (p.status) atomicOr(p.status, CA_STATUS_LENS);
     return -1;
   }
   if (b < 0 || b >= p.num_blocks) {
-    if (p.status) atomicOr(p.status, CA_STATUS_TABLE);
+    const bool freed = p.left >= 0 && pg * p.page >= p.sinks && (pg + 1) * p.page <= len - 1 - p.left;
+    if (p.status && !freed) atomicOr(p.status, CA_STATUS_TABLE);
     return -1;
   }
   return b;
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, kAppendCtas) append_8bit_ke
         if (k * ROWS < rows) held[k] = __ldg(reinterpret_cast<const uint4*>(at));
       }
     }
-    const int b = append_block(p, i, pg, id);
+    const int b = append_block(p, pg, id, (long long)before + n);
     if (b < 0) continue;
     float* scale = (side ? p.vs : p.ks) + (long long)b * p.H + h;
     uint8_t* block = static_cast<uint8_t*>(side ? p.vc : p.kc) + ((long long)b * p.H + h) * p.page * E;
@@ -348,7 +351,8 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
   if (before < 0) return;
   const long long pos = (long long)before + j;
   const long long pg = pos / p.page;
-  const int b = append_block(p, (int)i, pg, pg < p.pt_stride ? __ldg(p.page_table + i * p.pt_stride + pg) : -1);
+  const int b = append_block(p, pg, pg < p.pt_stride ? __ldg(p.page_table + i * p.pt_stride + pg) : -1,
+                             (long long)before + p.n_new);
   if (b < 0) return;
   const int off = (int)(pos - pg * p.page);
   const long long src = i * p.seq_stride + j * p.token_stride + (long long)h * E + v * VEC;

@@ -83,6 +83,7 @@ int append_plan(ca::AppendParams* prm, const void* key, const void* value, int64
   const int64_t pages = cu ? total / page + 2 * batch : (n_new + page - 2) / page + 1;
   if (pages > 0x7fffffffLL) return CA_EUNSUPPORTED;
   prm->pages = (int)pages;
+  prm->left = -1;
   prm->status = status;
   return CA_OK;
 }
@@ -191,6 +192,8 @@ int ca_decode_split(const void* q, int64_t q_stride, void* k_cache, void* v_cach
                      v_scale, num_blocks, lens, page_table, table_width, batch, kv_heads, head_dim, page, q_dtype,
                      status, &vec16);
     if (rc) return rc;
+    prm.left = window_left;
+    prm.sinks = sink_tokens;
     if ((rc = append(prm, head_dim, q_dtype, eight, vec16, s))) return rc;
   }
   ca::SplitCall c{};

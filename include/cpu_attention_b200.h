@@ -283,7 +283,11 @@ CA_API int ca_append_8bit(const void* key, const void* value, int64_t seq_stride
  * window_left and t < sink_tokens; pages wholly between them are not looked up,
  * their table entries may be anything. window_left -1: all L tokens.
  * n_new > 0: the new tokens k_new/v_new (q's dtype, kv_token_stride elements
- * apart) are appended at lens[i] first and L = lens[i] + n_new.
+ * apart) are appended at lens[i] first and L = lens[i] + n_new. They are written
+ * wherever their page's entry names a block, so the entries of pages that get
+ * new tokens have to be the sequence's own; where such a page lies wholly
+ * between the first tokens and the window, an entry outside the pool (-1)
+ * leaves its tokens out.
  * workspace: ca_decode_split_workspace_bytes() bytes, 16-byte aligned; its
  * content needs no preparation and is not kept between calls, but calls that
  * overlap in time must not share one. status: NULL or a device int32.

@@ -874,3 +874,55 @@ def test_prefill_packed_rows_of_others(dtype, hd, causal):
             out, lse = call(kk, vv)
             assert torch.equal(out[rows_q], want[rows_q]) and torch.equal(lse[:, rows_q], want_lse[:, rows_q])
     assert status() == 0
+
+
+@pytest.mark.parametrize("kind", ["8bit", "bf16", "fp32"])
+@pytest.mark.parametrize("n,left,sinks", [(60, 20, 4), (100, 0, 0), (33, 15, 17), (200, 70, 40)])
+def test_decode_appends_more_than_the_window(kind, n, left, sinks):
+    """New tokens that are behind the window at once: stored where the table names their page, left out where the page
+    is freed already (an entry outside the pool); the row is the same, and nothing is flagged."""
+    C = api()
+    lens, h, hk, d, page = [0, 15, 16, 100, 31], 4, 2, 64, 16
+    dtype = FP32 if kind == "fp32" else BF16
+    pc = S.Paged(kind, lens, hk, d, page, dtype, seed=n, room=n)
+    for c in (pc.k_cache, pc.v_cache) if kind == "8bit" else ():
+        u = c.view(torch.uint8)
+        u[(u & 0x7f) == 0x7f] = 0
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(len(lens), n, hk, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    q = torch.randn(len(lens), 1, h, d, generator=g).to(dtype).to(DEV)
+    opts = dict(window_size=(left, 0), sink_tokens=sinks)
+    start = [t for t in (pc.k_cache, pc.v_cache, pc.k_scale, pc.v_scale) if t is not None]
+    names = ["k_cache", "v_cache", "k_descale", "v_descale"][:len(start)]
+    outs, ends = [], []
+    table = pc.bt.clone()
+    freed = torch.zeros(table.shape, dtype=torch.bool)
+    for i, m in enumerate(lens):
+        for p in range(table.shape[1]):
+            freed[i, p] = p * page >= sinks and (p + 1) * page <= m + n - 1 - left
+    for bad in (None, -1, 0x7fffffff):
+        bt = table if bad is None else table.masked_fill(freed.to(DEV), bad)
+        caches = dict(zip(names, [t.clone() for t in start]))
+        outs.append(C.flash_attn_with_kvcache(q, k=k, v=v, cache_seqlens=pc.L, page_table=bt, **caches, **opts))
+        assert status() == 0
+        ends.append([bytes_of(t) for t in caches.values()])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    # with every page named, all tokens are there: a longer window finds them
+    stored = dict(zip(names, [t.clone() for t in start]))
+    full = C.flash_attn_with_kvcache(q, k=k, v=v, cache_seqlens=pc.L, page_table=table, **stored,
+                                     **({} if kind == "8bit" else dict(sink_tokens=0)))
+    assert all(torch.equal(a, bytes_of(b)) for a, b in zip(ends[0], stored.values()))
+    assert torch.isfinite(full).all()
+    # what is left out: the freed pages keep what they held
+    gone = table[freed.to(DEV)].long().cpu()
+    for a, b, was in zip(ends[1], ends[2], start):
+        assert torch.equal(a, b) and torch.equal(a[gone], bytes_of(was)[gone])
+    kept = torch.ones(start[0].shape[0], dtype=torch.bool)
+    kept[gone] = False
+    assert all(torch.equal(a[kept], b[kept]) for a, b in zip(ends[0], ends[1]))
+    # a bad entry of a page that is seen is flagged as ever
+    first = (lens[3] + n - 1) // page
+    table[3, first] = -1
+    C.flash_attn_with_kvcache(q, k=k, v=v, cache_seqlens=pc.L, page_table=table,
+                              **dict(zip(names, [t.clone() for t in start])), **opts)
+    assert status() == kernel().STATUS_TABLE
