@@ -121,7 +121,9 @@ def append_quantized(key, value, k_cache, v_cache, k_descale, v_descale, cache_s
     (448). It only grows while the block fills -- then the codes in it are
     rounded to the new scale, which loses nothing but what falls below the
     smallest code -- and starts afresh when a token is written at the block's
-    position 0. An infinity is stored as the largest code, NaN as NaN. A partly
+    position 0. A scale of the caller's own stays as long as it is large enough;
+    where one that is no power of two has to grow, codes move by up to half of
+    their step. An infinity is stored as the largest code, NaN as NaN. A partly
     filled block that sequences share has to be copied (``copy_blocks``) before
     one of them appends to it.
     """

@@ -109,7 +109,11 @@ class Paged:
     """Random paged caches: every sequence has its blocks in a shuffled order, and what no sequence uses -- slots past
     a length, blocks of nobody, pages behind a window -- holds NaN; freed table entries hold garbage."""
 
-    def __init__(self, kind, lens, kv_heads, d, page, dtype, seed=0, left=-1, sinks=0, room=0, device="cuda"):
+    def __init__(self, kind, lens, kv_heads, d, page, dtype, seed=0, left=-1, sinks=0, room=0, device="cuda", own=None,
+                 even=False):
+        # own: whether an 8-bit cache's scales are no powers of two (a user's own); by the seed when None.
+        # even: its values are near N(0, 1), so that scores differ by a few units and many keys carry weight.
+        own = bool(seed % 2) if own is None else own
         g = torch.Generator().manual_seed(seed)
         self.kind, self.lens, self.page, self.left, self.sinks = kind, list(lens), page, left, sinks
         ends = [-(-(n + room) // page) if n >= 0 else 0 for n in lens]
@@ -126,9 +130,13 @@ class Paged:
         if kind == "8bit":
             dt = F8
             for x in range(2):
-                s = torch.exp2(torch.randint(-9, 3, (total, kv_heads), generator=g).double())
+                s = torch.exp2(torch.randint(*((-1, 2) if even else (-9, 3)), (total, kv_heads), generator=g).double())
                 rows[x] = round_e4m3(rows[x] * 100)
-                self.scale[x] = s / 100 if seed % 2 else s  # powers of two, or a user's own
+                if even:
+                    s = s * (1.28 if own else 1) / 128
+                else:
+                    s = s / 100 if own else s
+                self.scale[x] = s
                 self.scale[x] = self.scale[x].float().double()
         else:
             dt = dtype

@@ -926,3 +926,88 @@ def test_decode_appends_more_than_the_window(kind, n, left, sinks):
     C.flash_attn_with_kvcache(q, k=k, v=v, cache_seqlens=pc.L, page_table=table,
                               **dict(zip(names, [t.clone() for t in start])), **opts)
     assert status() == kernel().STATUS_TABLE
+
+
+# ------------------------------------------------ scales of a user's own -----
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("d,page,h,hk", [(32, 16, 4, 4), (64, 64, 6, 2), (128, 16, 8, 1), (128, 48, 20, 2)])
+def test_decode_8bit_even_weights(dtype, own, d, page, h, hk):
+    """Scores a few units apart, so that outputs are sums over many keys and joins carry weight; scales that are powers
+    of two and ones that are not."""
+    lens = LENS + [4100]
+    pc = S.Paged("8bit", lens, hk, d, page, dtype, seed=d + page, own=own, even=True)
+    assert own == bool((torch.frexp(pc.scale[0])[0] != 0.5).any())
+    q = torch.randn(len(lens), 1, h, d, generator=torch.Generator().manual_seed(h)).to(dtype).to(DEV)
+    out, lse = api().flash_attn_with_kvcache(q, pc.k_cache, pc.v_cache, cache_seqlens=pc.L, page_table=pc.bt,
+                                             return_softmax_lse=True, **pc.opts())
+    S.check_decode(out, lse, q, pc, h)
+    assert status() == 0
+
+
+def check_append_own(cache, scale, codes, scales, rows, lens, table, page):
+    """One append where scales need not be powers of two: scales exactly, codes as near as the definition's roundings.
+    A quotient x / s, or a ratio and its product with a code, is rounded to fp32 (half a step 2^-24 each) before it is
+    rounded to a code: the code is within half a code's step, and 2^-23 of itself, of the exact quotient."""
+    want = codes.clone(), scales.clone()
+    exact = codes.clone()
+    for i, n in enumerate(lens):
+        r = rows[i]
+        for p in range(n // page, -(-(n + r.shape[0]) // page)):
+            a, z = max(n, p * page), min(n + r.shape[0], (p + 1) * page)
+            b = table[i][p]
+            for x in range(codes.shape[1]):
+                old = 0.0 if a == p * page else scales[b, x].item()
+                now = max(old, S.fit_scale(r[a - n:z - n, x]))
+                want[1][b, x] = now
+                if a != p * page and now != old:
+                    exact[b, x] = codes[b, x] * old / now
+                exact[b, x, a - p * page:z - p * page] = r[a - n:z - n, x] / now
+    got = cache.cpu().double()
+    _, e = torch.frexp(exact)
+    half = torch.exp2((e - 5).clamp(min=-10).double())  # of the step at the exact value
+    half = torch.where(exact.abs() > 448, math.inf, half)
+    assert torch.equal(scale.cpu().double(), want[1])
+    err = (got - exact).abs()
+    assert (err <= half + exact.abs() * 2.0 ** -23).all(), (err - half).max().item()
+    return got, want[1]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 32), (32, 48)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_append_to_scales_of_a_users_own(dtype, d, page, packed):
+    """Calibrated scales stay while they are large enough and codes are rounded to them; where they are too small the
+    scale grows and the block's codes are rounded by a ratio that is no power of two; the row attended is the cache's."""
+    g = torch.Generator().manual_seed(d + packed)
+    heads, lens, width = 3, [5, page - 1, 2 * page - 3, page, 3], 4
+    table = torch.randperm(5 * width + 2, generator=g)[:5 * width].reshape(5, width).to(torch.int32)
+    blocks = 5 * width + 2
+    caches = [S.round_e4m3(torch.randn(blocks, heads, page, d, generator=g, dtype=torch.float64) * 100) for _ in range(2)]
+    scales = [torch.rand(blocks, heads, generator=g).mul(0.4).add(0.03).double() for _ in range(2)]
+    scales[0][table[0][0]] = torch.tensor([0.37, 1e-3, 3e-38]).double()  # kept, grown, grown from next to nothing
+    scales[1][table[1][0]] = torch.tensor([1e30, 0.0, 0.37]).double()
+    scales = [s.float().double() for s in scales]
+    kc, vc = (c.float().to(S.F8).to(DEV) for c in caches)
+    ks, vs = (s.float().to(DEV) for s in scales)
+    for n, size in ((1, 1.0), (3, 30.0), (page + 2, 3000.0)):
+        k, v = (torch.randn(5, n, heads, d, generator=g).mul(size).to(dtype) for _ in range(2))
+        more = {}
+        args = (k.to(DEV), v.to(DEV))
+        if packed:
+            args = tuple(t.flatten(0, 1) for t in args)
+            more = dict(cu_seqlens_new=torch.arange(0, 5 * n + 1, n, dtype=torch.int32, device=DEV), max_seqlen_new=n)
+        api().append_quantized(*args, kc, vc, ks, vs, torch.tensor(lens, dtype=torch.int32, device=DEV), table.to(DEV),
+                               **more)
+        for x, (r, c, s) in enumerate(((k, kc, ks), (v, vc, vs))):
+            caches[x], scales[x] = check_append_own(c, s, caches[x], scales[x], [t.double() for t in r], lens,
+                                                    table.tolist(), page)
+        lens = [a + n for a in lens]
+    assert status() == 0
+    q = torch.randn(5, 1, 6, d, generator=g).to(dtype).to(DEV)
+    pc = S.Paged("8bit", lens, heads, d, page, dtype, own=True)
+    pc.table, pc.rows, pc.scale = table.tolist(), caches, scales
+    out, lse = api().flash_attn_with_kvcache(q, kc, vc, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                             page_table=table.to(DEV), k_descale=ks, v_descale=vs, softmax_scale=1e-3,
+                                             return_softmax_lse=True)
+    S.check_decode(out, lse, q, pc, 6, scale=1e-3)
