@@ -130,7 +130,7 @@ def append_quantized(key, value, k_cache, v_cache, k_descale, v_descale, cache_s
     args = (key, value, k_cache, v_cache, k_descale, v_descale, cache_seqlens, page_table, cu_seqlens_new)
     most = 0
     if cu_seqlens_new is not None:
-        most = key.shape[0] if max_seqlen_new is None else int(max_seqlen_new)
+        most = key.shape[0] if max_seqlen_new is None else min(int(max_seqlen_new), key.shape[0])
     if _native.append_8bit(0, *args, most) is not None:
         return
     args = _explain_append(*args, most)

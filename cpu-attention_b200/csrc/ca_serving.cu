@@ -134,7 +134,8 @@ int ca_append_8bit(const void* key, const void* value, int64_t seq_stride, int64
   if (!head_dim_ok(head_dim)) return CA_EHEADDIM;
   if (!page_ok(page)) return CA_EPAGE;
   if (!sizes_ok(batch, heads, num_blocks, table_width, n_new) || total_new < 0) return CA_ESHAPE;
-  if (batch == 0 || n_new == 0 || (cu_new && total_new == 0)) return CA_OK;
+  // (packed tokens with n_new = 0 go on: a sequence that has some is flagged)
+  if (batch == 0 || (cu_new ? total_new == 0 : n_new == 0)) return CA_OK;
   if (num_blocks && (!k_scale || !v_scale)) return CA_ENULL;
   if (!aligned(k_scale, 4) || !aligned(v_scale, 4)) return CA_ELAYOUT;
   ca::AppendParams prm{};

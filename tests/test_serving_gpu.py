@@ -1011,3 +1011,27 @@ def test_append_to_scales_of_a_users_own(dtype, d, page, packed):
                                              page_table=table.to(DEV), k_descale=ks, v_descale=vs, softmax_scale=1e-3,
                                              return_softmax_lse=True)
     S.check_decode(out, lse, q, pc, 6, scale=1e-3)
+
+
+def test_append_packed_stated_maximum():
+    """The stated longest sequence may be any number: too small a one is flagged (0, too), a huge one is no limit."""
+    C, K = api(), kernel()
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(20, 2, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    cu = torch.tensor([0, 5, 20], dtype=torch.int32, device=DEV)
+    L = torch.zeros(2, dtype=torch.int32, device=DEV)
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device=DEV)
+    want = empty_8bit(4, 2, 16, 64, 0)
+    C.append_quantized(k, v, *want, L, table, cu)
+    assert status() == 0 and (want[2] > 0).sum() == 4
+    for most, flag in ((15, 0), (1 << 40, 0), (0, K.STATUS_LENS), (4, K.STATUS_LENS)):
+        got = empty_8bit(4, 2, 16, 64, 0)
+        C.append_quantized(k, v, *got, L, table, cu, most)
+        assert status() == flag, most
+        if not flag:
+            assert all(torch.equal(bytes_of(a), bytes_of(b)) for a, b in zip(got, want))
+        elif most == 0:
+            assert all((bytes_of(a) == 0).all() for a in got)
+    with pytest.raises(ValueError):
+        C.append_quantized(k, v, *want, L, table, cu, -1)
+    assert status() == 0
