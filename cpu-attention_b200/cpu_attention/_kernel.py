@@ -141,6 +141,7 @@ def cuda_error():
 # zero between calls (the kernel leaves them so), so a workspace is zero-filled
 # when it is made. Calls on one stream are ordered, so they may share one.
 _WS = {}
+_WS_OUTGROWN = []
 _WS_LOCK = threading.Lock()
 _MIN_WS = 1 << 16
 
@@ -179,6 +180,8 @@ def workspace(device, stream, nbytes=0):
             ws = _WS.get(key)
             if ws is None or ws.numel() < nbytes:
                 size = max(nbytes, _MIN_WS, 0 if ws is None else 2 * ws.numel())
+                if ws is not None:
+                    _WS_OUTGROWN.append(ws)  # a captured graph may hold its address
                 ws = torch.zeros(size, dtype=torch.uint8, device=device)
                 _WS[key] = ws
     return ws

@@ -31,10 +31,12 @@ namespace {
 
 std::mutex g_ws_mutex;
 std::map<std::pair<int, uintptr_t>, at::Tensor> g_ws;
+std::vector<at::Tensor> g_ws_outgrown;  // (sizes double: no more bytes than those in use)
 constexpr int64_t kMinWorkspace = 1 << 16;
 
 // The workspace tensor of (device, stream), at least nbytes long, zero-filled
-// when made (the decode kernel leaves its tickets and counter at zero).
+// when made (the decode kernel leaves its tickets and counter at zero). One that
+// has been outgrown stays: a captured graph may hold its address.
 at::Tensor workspace(int64_t device, uintptr_t stream, int64_t nbytes) {
   std::lock_guard<std::mutex> lock(g_ws_mutex);
   const auto key = std::make_pair((int)device, stream);
@@ -43,6 +45,7 @@ at::Tensor workspace(int64_t device, uintptr_t stream, int64_t nbytes) {
   const int64_t grown = it == g_ws.end() ? 0 : 2 * it->second.numel();
   const int64_t size = std::max({nbytes, kMinWorkspace, grown});
   at::Tensor ws = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
+  if (it != g_ws.end()) g_ws_outgrown.push_back(it->second);
   g_ws[key] = ws;
   return ws;
 }

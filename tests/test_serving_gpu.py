@@ -1035,3 +1035,41 @@ def test_append_packed_stated_maximum():
     with pytest.raises(ValueError):
         C.append_quantized(k, v, *want, L, table, cu, -1)
     assert status() == 0
+
+
+# --------------------------------------------------- workspaces and graphs -----
+def small_decode(seed):
+    """A decode whose items are split (its joins use the workspace), over float caches."""
+    g = torch.Generator().manual_seed(seed)
+    kc, vc = (torch.randn(80, 4, 16, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    bt = torch.randperm(80, generator=g).to(torch.int32).view(2, 40).to(DEV)
+    L = torch.tensor([640, 333], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 1, 4, 64, generator=g).bfloat16().to(DEV)
+    return lambda: api().flash_attn_with_kvcache(q, kc, vc, cache_seqlens=L, page_table=bt)
+
+
+def test_outgrown_workspace_stays_for_graphs():
+    """A graph holds its workspace's address; a larger call on the stream gets a new one and the old one stays."""
+    K = kernel()
+    stream = torch.cuda.Stream()
+    dev = torch.device("cuda", torch.cuda.current_device())
+    call = small_decode(3)
+    with torch.cuda.stream(stream):
+        want = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = call()
+    with torch.cuda.stream(stream):
+        old = K.workspace(dev, stream.cuda_stream)
+        address, size = old.data_ptr(), old.numel()
+        del old
+        assert K.workspace(dev, stream.cuda_stream, size + 1).data_ptr() != address
+        others = [torch.full((size,), 0x5a, dtype=torch.uint8, device=DEV) for _ in range(8)]
+        assert all(t.data_ptr() >= address + size or t.data_ptr() + size <= address for t in others)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+        assert all(bool((t == 0x5a).all()) for t in others)
+        assert torch.equal(call(), want)
