@@ -34,6 +34,27 @@ std::map<std::pair<int, uintptr_t>, at::Tensor> g_ws;
 std::vector<at::Tensor> g_ws_outgrown;  // (sizes double: no more bytes than those in use)
 constexpr int64_t kMinWorkspace = 1 << 16;
 
+// Zeros that are there before this returns when the current stream is capturing:
+// made in the graph they would be zeros only once that graph has run, and the
+// next graph captured on the stream, or a call outside, may come first.
+at::Tensor zeroed(int64_t device, int64_t size) {
+  const auto options = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+    return at::zeros({size}, options);
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  for (int tries = 0; tries < 64; ++tries) {
+    const c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)device);
+    cudaStreamCaptureStatus status;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(side.stream(), &status));
+    if (status != cudaStreamCaptureStatusNone) continue;  // (the pool hands its streams out in turn)
+    const c10::cuda::CUDAStreamGuard guard(side);
+    at::Tensor ws = at::zeros({size}, options);
+    C10_CUDA_CHECK(cudaStreamSynchronize(side.stream()));
+    return ws;
+  }
+  throw std::runtime_error("cpu_attention: every stream is being captured");
+}
+
 // The workspace tensor of (device, stream), at least nbytes long, zero-filled
 // when made (the decode kernel leaves its tickets and counter at zero). One that
 // has been outgrown stays: a captured graph may hold its address.
@@ -44,7 +65,7 @@ at::Tensor workspace(int64_t device, uintptr_t stream, int64_t nbytes) {
   if (it != g_ws.end() && it->second.numel() >= nbytes) return it->second;
   const int64_t grown = it == g_ws.end() ? 0 : 2 * it->second.numel();
   const int64_t size = std::max({nbytes, kMinWorkspace, grown});
-  at::Tensor ws = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
+  at::Tensor ws = zeroed(device, size);
   if (it != g_ws.end()) g_ws_outgrown.push_back(it->second);
   g_ws[key] = ws;
   return ws;

@@ -1048,6 +1048,30 @@ def small_decode(seed):
     return lambda: api().flash_attn_with_kvcache(q, kc, vc, cache_seqlens=L, page_table=bt)
 
 
+def test_workspace_made_in_a_capture_is_zero_before_the_replay():
+    """A stream's first call may be a captured one: what it leaves for the calls behind it does not wait for that
+    graph's first replay. Graphs of one stream give the same in any order of replay."""
+    K = kernel()
+    stream = torch.cuda.Stream(priority=-1)  # (of a pool that nothing here has used)
+    dev = torch.device("cuda", torch.cuda.current_device())
+    first, second = small_decode(1), small_decode(2)
+    want = first(), second()
+    torch.cuda.synchronize()
+    graphs = []
+    for call in (first, second):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = call()
+        graphs.append((graph, out))
+        assert int(K.workspace(dev, stream.cuda_stream).count_nonzero()) == 0
+    with torch.cuda.stream(stream):
+        assert torch.equal(second(), want[1])
+        for i in (1, 0, 1):
+            graphs[i][0].replay()
+            assert torch.equal(graphs[i][1], want[i])
+        assert status() == 0
+
+
 def test_outgrown_workspace_stays_for_graphs():
     """A graph holds its workspace's address; a larger call on the stream gets a new one and the old one stays."""
     K = kernel()
