@@ -25,7 +25,8 @@ from .cache import check_eight_bit, check_packed_caches, packed_rows, reshape_an
 
 # flash_attn_with_kvcache options no kernel here implements; setting one raises
 _NOT_SUPPORTED = ("cpu_attention: qv, rotary, cache_leftpad, varlen, descale of float caches, sliding windows without "
-                  "sink_tokens, softcap, attention_chunk and alibi are not supported")
+                  "sink_tokens (give sink_tokens=0 for a window alone), softcap, attention_chunk and alibi are not "
+                  "supported")
 
 
 def _as_tensor(x):
@@ -114,7 +115,9 @@ def flash_attn_with_kvcache(
     ``append_quantized`` or ``k``/``v`` here, both sides ``[num_blocks,
     nheads_k, page_block_size, headdim]`` without a transpose) come with
     ``k_descale`` and ``v_descale``, float32 ``[num_blocks, nheads_k]``: a value
-    is its code times its block's and head's scale. ``q`` (and ``k``/``v``) stay
+    is its code times its block's and head's scale. (flash-attn's arguments of
+    these names are ``[batch, nheads_k]``, one scale per sequence; scales laid
+    out so do not belong here, also where the two shapes happen to be equal.) ``q`` (and ``k``/``v``) stay
     fp32 or bf16; appending updates caches and scales.
 
     ``sink_tokens`` (0 or more) turns ``window_size`` on, for float and 8-bit
@@ -124,7 +127,7 @@ def flash_attn_with_kvcache(
     be anything (``compact_blocks`` frees them), but for pages that get tokens
     of ``k``/``v``: those are written wherever the entry names a block, and left
     out in such a page where it is -1. Without ``sink_tokens`` a window is
-    refused, as in the reference.
+    refused, as in the reference; ``sink_tokens=0`` is a window alone.
     """
     # (every option at its default: the common case, decided without building
     # the option table -- an engine calls this once per layer and token)

@@ -284,3 +284,12 @@ def test_step_example_packs_with_the_new_token_counted(monkeypatch):
     names = dict.fromkeys("q k v k_cache v_cache k_scale v_scale table".split())
     exec(step_example(), dict(names, lens=lens, page=16))
     assert seen["attend"].tolist() == [16, 5] and seen["pack"].tolist() == [17, 6]
+
+
+def test_refused_window_names_the_way():
+    """A window alone is the reference's refusal; its message says how to have one."""
+    q, kc, vc, bt, ks, vs = eight()
+    f = torch.zeros(4, 2, 16, 64)
+    for caches in ((f, f.clone(), {}), (kc, vc, dict(k_descale=ks, v_descale=vs))):
+        with pytest.raises(NotImplementedError, match="sink_tokens=0"):
+            C.flash_attn_with_kvcache(q, *caches[:2], cache_seqlens=4, page_table=bt, window_size=(8, 0), **caches[2])
