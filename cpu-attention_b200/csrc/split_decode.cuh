@@ -121,14 +121,14 @@ struct SplitSeq {
 
 __device__ __forceinline__ SplitSeq split_seq(const SplitParams& p, int i) {
   SplitSeq s;
-  long long L = (long long)__ldg(p.lens + i) + p.extra;
+  const int before = __ldg(p.lens + i);
+  // a negative length is a sequence that is skipped
+  long long L = before < 0 ? 0LL : (long long)before + p.extra;
   const long long cap = p.pt_stride * (long long)p.page;
   if (L > cap) {
     if (p.status) atomicOr(p.status, CA_STATUS_LENS);
     L = cap;
   }
-  // a negative length is a sequence that is skipped
-  if (__ldg(p.lens + i) < 0) L = 0;
   s.L = (int)L;
   const int all = (s.L + kSplitTile - 1) / kSplitTile;
   s.low = 0;

@@ -1097,3 +1097,22 @@ def test_outgrown_workspace_stays_for_graphs():
             assert torch.equal(out, want)
         assert all(bool((t == 0x5a).all()) for t in others)
         assert torch.equal(call(), want)
+
+
+@pytest.mark.parametrize("kind", ["8bit", "bf16", "fp32"])
+def test_decode_append_skips_negative_lengths_without_a_flag(kind):
+    """A sequence left out by a negative length takes no new tokens, however many there are for it."""
+    dtype = FP32 if kind == "fp32" else BF16
+    pc = S.Paged(kind, [3, -1, -1], 2, 64, 16, dtype, seed=2, room=10)
+    for c in (pc.k_cache, pc.v_cache) if kind == "8bit" else ():
+        u = c.view(torch.uint8)
+        u[(u & 0x7f) == 0x7f] = 0
+    before = [bytes_of(c) for c in (pc.k_cache, pc.v_cache)]
+    q = torch.ones(3, 1, 4, 64, dtype=dtype, device=DEV)
+    new = torch.ones(3, 40, 2, 64, dtype=dtype, device=DEV)
+    status()
+    out, lse = api().flash_attn_with_kvcache(q[1:], pc.k_cache, pc.v_cache, k=new[1:], v=new[1:], cache_seqlens=pc.L[1:],
+                                             page_table=pc.bt[1:], sink_tokens=0, return_softmax_lse=True, **pc.opts())
+    assert status() == 0
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    assert all(torch.equal(bytes_of(c), b) for c, b in zip((pc.k_cache, pc.v_cache), before))
