@@ -15,9 +15,12 @@
 // One warp owns a (sequence, touched page, head) of K or of V: it is the only
 // writer of that block and scale, so there are no atomics and the result does
 // not depend on order. Bound by HBM (2 bytes read and 1 written per value at
-// bf16) for prompts: 24.6k tokens of 16 heads of 128 dims, 302 MB, in 49 us (6.2
-// TB/s, 94% of the measured copy rate). One token per sequence is a launch and
-// three loads that wait for one another (length, block id, scale): 2.8 us.
+// bf16) for prompts: 24.6k tokens of 16 heads of 128 dims, 302 MB, in 49 us
+// replayed from a graph (6.2 TB/s, 94% of the measured copy rate), 51 to 54 us
+// as calls of their own whose inputs change (85 to 90%); fp32 tokens, 504 MB, in
+// 101 us (5.0 TB/s: a lane holds 8 of a 16-token page's 16 vectors and loads the
+// rest twice). One token per sequence is a launch and three loads that wait for
+// one another (length, block id, scale): 2.6 us.
 //
 // append_rows_kernel: the same places in a float cache, bit-exact (the layout
 // of store.cuh), any number of tokens per sequence.
@@ -129,7 +132,7 @@ __device__ __forceinline__ void append_load(float (&x)[VEC], const T* p) {
 
 constexpr int kAppendWarps = 4;
 // 8 CTAs an SM (64 registers, nothing of bf16 spilled) keep enough loads in flight:
-// prompts 49.1 us; 6 CTAs 55.1, as many as the registers would leave (5) 58.4,
+// prompts 49.1 us (graph replay, as all of these); 6 CTAs 55.1, as many as the registers would leave (5) 58.4,
 // 10 (held vectors spill) 55.2. One token a sequence does not fill an SM and loses
 // 0.1 us to the tighter schedule.
 constexpr int kAppendCtas = 8;

@@ -5,7 +5,8 @@
 // copies one block of one tensor, or (blocks up to 1 KiB: scales) 64 pairs of it.
 // Bound by HBM: each byte read and written once; 8 words a thread in flight
 // (4 at twice the warps: 44 us; 512 threads: 48 us; 128: 34 us). 65 blocks of 48
-// tensors (204 MB both ways) in 33 us, 6.1 TB/s.
+// tensors (204 MB both ways) in 34 us, 6.0 TB/s. Few large blocks leave most SMs
+// without work: one pair of 1 MiB blocks in 30 tensors takes 33 us.
 //
 // compact_plan_kernel (one CTA): with U the blocks that the page table's rows
 // use and n = |U|, the k-th smallest member of U that is >= n goes to the k-th
@@ -14,7 +15,9 @@
 // several rows share moves once. U is a bitmap in shared memory; ranks are
 // prefix sums of its population counts. A pool of 2111 blocks is planned in 9.5
 // us; with its moves (24 8-bit caches and their scales, 387 MB) 70 us (a move's ids
-// loaded only once the last one's bytes are written: 77 us).
+// loaded only once the last one's bytes are written: 77 us). What does not fit the
+// CTA's registers of a table (4096 entries) is read twice by this one CTA: 256 x
+// 2048 entries take 587 us in all, their moves' bytes 16 of them.
 #pragma once
 
 #include "common.cuh"

@@ -20,7 +20,9 @@
 // which about 6 us pass before the first tile is in (lengths, block ids and
 // scales, tiles: round trips that wait for one another) and 5 us behind the
 // last one (the join); 8-bit tiles are then bound by latency of the chain
-// widen, multiply, weigh (40% of issue slots used), not by HBM.
+// widen, multiply, weigh (40% of issue slots used), not by HBM. fp32 caches
+// behind a window of 4096, 32 sequences, 32 / 8 heads of 128: 229 us for 0.99 GB
+// (4.3 TB/s); heads of 64: 257 us, of 32: 351 us for as many bytes.
 //
 // Work: the visible tokens of every item (sequence, KV head, up to 8 of its
 // query heads) are cut into tiles of 16 tokens (more for small head_dims); pages
@@ -47,11 +49,11 @@
 //   weight, against 2^-9 of the output's rounding) and as a value plus its rest
 //   for fp32 ones and for bf16 caches; s_v enters with it, its exponent with the
 //   weight's, so any scales a user stores are followed.
-// fp32 caches run the same tiles on FMAs.
+// fp32 caches run the same tiles on FMAs, through a ring in shared memory.
 //
-// Loads of tile n+1 are issued as soon as the registers of tile n are free: 12
-// warps an SM with a tile each in flight are 48 KiB, about twice what HBM's
-// latency asks for; 8-bit tiles are called into L2 one tile earlier still (-8%;
+// 8-bit and bf16 caches: loads of tile n+1 are issued as soon as the registers of
+// tile n are free: 12 warps an SM with a tile each in flight are 48 KiB, about
+// twice what HBM's latency asks for; 8-bit tiles are called into L2 one tile earlier still (-8%;
 // four tiles earlier: +4%, eight: +17%). Measured against this (8-bit grouped,
 // 96 us then): cp.async into shared memory with four tiles ahead 132 us, TMA
 // tiles swizzled for conflict-free fragment loads 96 us, two tiles ahead in
@@ -70,7 +72,10 @@ namespace ca {
 enum SplitKind { kSplitF32 = 0, kSplitBf16 = 1, kSplitE4m3 = 2 };
 
 constexpr int kSplitWarps = 6;        // warps per CTA
-constexpr int kSplitCtasPerSm = 2;    // CTAs per SM
+// CTAs per SM of the grid. Two of the 8-bit and bf16 kinds fit; one of the fp32
+// kind (130 to 185 KB of shared memory: rings, query rows, pieces), whose grid
+// runs as two rounds.
+constexpr int kSplitCtasPerSm = 2;
 constexpr int kSplitTile = 16;        // tokens per tile
 constexpr int kSplitMaxBatch = 1024;  // sequences per launch (their tile counts sit in shared memory)
 constexpr int kSplitRing = 16384;     // fp32 caches: bytes of tiles a warp has in flight
