@@ -257,7 +257,7 @@ def test_compact_reserved_lengths_refusals():
 
 
 def step_example():
-    """The decode step with compaction that INTEGRATION.md shows, as code."""
+    """The decode step with compaction that the integration guide shows, as code."""
     import os
     import re
 

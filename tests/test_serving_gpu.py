@@ -818,7 +818,7 @@ def test_compact_keeps_what_is_seen_and_reserved(kind, left, sinks):
 
 
 def test_step_example_keeps_the_new_token():
-    """INTEGRATION.md's decode step with a compaction behind it, with lengths that end at a page: the next step finds
+    """The integration guide's decode step with a compaction behind it, with lengths that end at a page: the next step finds
     every token."""
     from test_serving_api import step_example
     C = api()
@@ -1116,3 +1116,105 @@ def test_decode_append_skips_negative_lengths_without_a_flag(kind):
     assert status() == 0
     assert (out == 0).all() and torch.isneginf(lse).all()
     assert all(torch.equal(bytes_of(c), b) for c, b in zip((pc.k_cache, pc.v_cache), before))
+
+
+# ------------------------------------------------- captured, and from threads -----
+def serving_step(seed):
+    """Prompts into 8-bit caches, a fork, a packing, a windowed decode with new tokens, a windowed prefill: a call of all
+    of them on fixed buffers, what fills the buffers, and what the call leaves."""
+    C = api()
+    hk, d, page, width, news = 2, 64, 16, 6, [30, 0, 47]
+    lens, total = [3, 16, 20], 77
+    g = torch.Generator().manual_seed(seed)
+    start = [t.to(DEV) for t in (torch.randint(0, 120, (24, hk, page, d), generator=g, dtype=torch.uint8),
+                                 torch.randint(0, 120, (24, hk, page, d), generator=g, dtype=torch.uint8),
+                                 torch.rand(24, hk, generator=g), torch.rand(24, hk, generator=g))]
+    caches = [t.clone() for t in start]
+    kc, vc = (c.view(S.F8) for c in caches[:2])
+    table = torch.randperm(24, generator=g)[:18].reshape(3, width).to(torch.int32)
+    spare = sorted(set(range(24)) - set(table.flatten().tolist()))
+    pairs = torch.tensor([[int(table[0, 0]), spare[0]], [int(table[2, 1]), spare[1]]], device=DEV)
+    cu = torch.tensor([0, 30, 30, 77], dtype=torch.int32, device=DEV)
+    L = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    table, after = table.to(DEV), L + torch.tensor(news, dtype=torch.int32, device=DEV)
+    k, v, q1, k1, v1 = (torch.empty(*s, d, dtype=BF16, device=DEV) for s in ((total, hk), (total, hk), (3, 1, 4),
+                                                                             (3, 1, hk), (3, 1, hk)))
+    q = torch.empty(total, 4, d, dtype=BF16, device=DEV)
+
+    def fill(r):
+        g = torch.Generator().manual_seed(1000 * seed + r)
+        for t in (k, v, q, q1, k1, v1):
+            t.copy_(torch.randn(t.shape, generator=g).bfloat16())
+        for t, was in zip(caches, start):
+            t.copy_(was)
+
+    def call():
+        C.append_quantized(k, v, kc, vc, *caches[2:], L, table, cu, 47)
+        C.copy_blocks([kc, vc, *caches[2:]], pairs)
+        new, used = C.compact_blocks([kc, vc, *caches[2:]], table, after, page, (40, 0), 4, after + 1)
+        out = C.flash_attn_with_kvcache(q1, kc, vc, k=k1, v=v1, cache_seqlens=after, page_table=new,
+                                        k_descale=caches[2], v_descale=caches[3], window_size=(40, 0), sink_tokens=4)
+        pre = C.flash_attn_varlen_func(q, k, v, cu, cu, 47, 47, causal=True, window_size=(20, 0), sink_tokens=2)
+        return [out, pre, new, used]
+
+    return fill, call, caches
+
+
+def test_serving_calls_captured_and_from_threads():
+    """The calls above captured on two streams and replayed side by side, and made by two threads at once on streams of
+    their own, give what they give one after the other."""
+    import threading
+    K = kernel()
+    steps = [serving_step(x) for x in (1, 2)]
+    want = []
+    for x, (fill, call, caches) in enumerate(steps):
+        want.append([])
+        for r in range(3):
+            fill(r)
+            want[x].append([t.clone() for t in call() + caches])
+    assert status() == 0
+    torch.cuda.synchronize()
+    graphs = []
+    for fill, call, caches in steps:
+        fill(0)
+        torch.cuda.synchronize()
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs = call()
+        graphs.append((stream, graph, outs))
+    for r in range(3):
+        for fill, _, _ in steps:
+            fill(r)
+        torch.cuda.synchronize()
+        for stream, graph, _ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, caches), (_, _, outs), w in zip(steps, graphs, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs + caches, w[r]))
+    for stream, _, _ in graphs:
+        with torch.cuda.stream(stream):
+            assert status() == 0
+    failed = []
+
+    def work(x):
+        fill, call, caches = steps[x]
+        stream = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(stream):
+                for r in range(30):
+                    fill(r % 3)
+                    got = call() + caches
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[x][r % 3])):
+                        failed.append((x, r))
+                if K.status(torch.device("cuda", torch.cuda.current_device())):
+                    failed.append((x, "status"))
+        except Exception as e:  # noqa: BLE001
+            failed.append((x, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(x,)) for x in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
