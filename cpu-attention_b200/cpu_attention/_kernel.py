@@ -215,7 +215,8 @@ def status(device=None, stream=None, reset=True):
 
 
 _STATUS_TEXT = [
-    (STATUS_LENS, ValueError, "cpu_attention: cache_seqlens exceed the page table's capacity"),
+    (STATUS_LENS, ValueError, "cpu_attention: cache_seqlens exceed the page table's capacity, or packed offsets their "
+                              "tokens"),
     (STATUS_SLOT, ValueError, "cpu_attention: slot_mapping points past the end of the cache"),
     (STATUS_TABLE, ValueError, "cpu_attention: page_table points past the end of the cache"),
     (STATUS_TIMEOUT, RuntimeError, "cpu_attention: a device wait timed out"),

@@ -462,6 +462,7 @@ int ca_flash_window(const void* q, const void* k, const void* v, void* out, floa
   prm.left = window_left < 0 ? -1 : (int)std::min(window_left, most);
   prm.right = causal ? 0 : (window_right < 0 ? -1 : (int)std::min(window_right, most));
   prm.sinks = prm.win ? (int)std::min(sink_tokens, seq_k) : 0;
+  prm.status = status;
   int device;
   int rc = current_device(&device);
   if (rc) return rc;

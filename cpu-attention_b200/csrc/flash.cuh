@@ -36,6 +36,7 @@ struct FlashParams {
   // position i + Lk - Lq, sees keys from `left` before it (and the first
   // `sinks` keys) to `right` after it; a negative side has no limit
   int win, left, right, sinks;
+  int* status;
 };
 
 // The keys row i of a windowed launch sees: j <= hi and (j >= lo or j < sinks).
@@ -60,14 +61,20 @@ struct FlashSeq {
   long long lbase;     // lse index of row 0 of head h
 };
 
+// Packed: offsets are brought into [0, total] and a sequence's end to its start
+// or later, and flagged, so that no bad one is followed out of the tensors.
 template <typename P>
 __device__ __forceinline__ FlashSeq flash_seq(const P& p, int b, int h, int E) {
   FlashSeq s;
   if (p.cu_q) {
-    s.tq0 = __ldg(p.cu_q + b);
-    s.tk0 = __ldg(p.cu_k + b);
-    s.Lq = __ldg(p.cu_q + b + 1) - (int)s.tq0;
-    s.Lk = __ldg(p.cu_k + b + 1) - (int)s.tk0;
+    const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1), k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
+    const int tq = min(max(q0, 0), (int)p.total_q), tk = min(max(k0, 0), (int)p.total_k);
+    s.Lq = min(max(q1, tq), (int)p.total_q) - tq;
+    s.Lk = min(max(k1, tk), (int)p.total_k) - tk;
+    if (tq != q0 || tq + s.Lq != q1 || tk != k0 || tk + s.Lk != k1)
+      if (p.status) atomicOr(p.status, CA_STATUS_LENS);
+    s.tq0 = tq;
+    s.tk0 = tk;
     s.obase = s.tq0 * p.H * E;
     s.lbase = (long long)h * p.total_q + s.tq0;
   } else {

@@ -43,6 +43,7 @@ struct FlashTcArgs {
   void* out;               // [B, Lq, H, E] contiguous (varlen: [total_q, H, E])
   float* lse;              // [B, H, Lq] (varlen: [H, total_q]) or NULL
   long long total_q;       // varlen: query tokens (the lse row length)
+  long long total_k;       // varlen: key tokens
   const int* cu_q;         // varlen sequence starts (see FlashParams), or NULL
   const int* cu_k;
   int B, Lq, Lk, H;        // varlen: Lq, Lk are the largest lengths
@@ -650,6 +651,7 @@ int flash_tc_launch(const FlashParams& p, int* status, cudaStream_t stream, std:
   a.out = p.out;
   a.lse = p.lse;
   a.total_q = p.total_q;
+  a.total_k = p.total_k;
   a.cu_q = p.cu_q;
   a.cu_k = p.cu_k;
   a.B = p.B;

@@ -54,7 +54,8 @@ extern "C" {
 #define CA_ESCRATCH -10     /* beyond ca_decode_noalloc's static scratch        */
 
 /* status bits written by the device into the workspace (ca_status) */
-#define CA_STATUS_LENS 1    /* cache_seqlens (+ the appended token) past W*page */
+#define CA_STATUS_LENS 1    /* cache_seqlens (+ the appended token) past W*page,
+                               or packed offsets that fall or leave the tokens  */
 #define CA_STATUS_TABLE 2   /* a page-table entry outside [0, num_blocks)      */
 #define CA_STATUS_SLOT 4    /* a slot_mapping entry >= num_blocks * page       */
 #define CA_STATUS_TIMEOUT 8 /* a bounded device wait gave up                   */
@@ -216,7 +217,9 @@ CA_API int ca_flash(const void* q, const void* k, const void* v, void* out,
  *   sequence lengths (no sequence may exceed them), the strides' batch entry
  *   is ignored, out is [total_q, heads, head_dim] and causal masks per
  *   sequence (bottom-right). total_q / total_k are ignored when dense. Rows of
- *   k/v of other sequences, or behind the last one, may hold anything.
+ *   k/v of other sequences, or behind the last one, may hold anything. Offsets
+ *   outside [0, total], or below the one before, count as the nearest that is
+ *   not, and are flagged (CA_STATUS_LENS).
  */
 CA_API int ca_flash_ex(const void* q, const void* k, const void* v, void* out,
              float* lse, int64_t batch, int64_t seq_q, int64_t seq_k,

@@ -1218,3 +1218,27 @@ def test_serving_calls_captured_and_from_threads():
     for t in threads:
         t.join()
     assert not failed
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("window", [(-1, -1), (5, 0), (-1, 9)])
+def test_prefill_packed_offsets_past_the_tokens(dtype, window):
+    """Offsets on the device that leave the packed tokens, or fall, are brought back and flagged: nothing is read or
+    written out of place, and the sequences that they do not concern are as ever."""
+    C, K = api(), kernel()
+    g = torch.Generator().manual_seed(1)
+    n = 330
+    q, k, v = (torch.randn(n, h, 64, generator=g).to(dtype).to(DEV) for h in (4, 2, 2))
+    cu = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    call = lambda cq, ck, causal: C.flash_attn_varlen_func(q, k, v, cq, ck, n, n, causal=causal,  # noqa: E731
+                                                           window_size=window, return_attn_probs=True)
+    for causal in (False, True):
+        for bad, good in (((0, 200, 1 << 30), (0, 200, n)), ((-7, 200, n), (0, 200, n)), ((0, 200, 120), (0, 200, 200)),
+                          ((0, 200, -(1 << 31)), (0, 200, 200)), ((0, 1 << 29, 1 << 30), (0, n, n))):
+            want, want_lse = call(cu(*good), cu(*good), causal)
+            assert status() == 0
+            for cq, ck in ((bad, good), (good, bad), (bad, bad)):
+                out, lse = call(cu(*cq), cu(*ck), causal)
+                assert status() == K.STATUS_LENS
+                rows = good[2]
+                assert torch.equal(out[:rows], want[:rows]) and torch.equal(lse[:, :rows], want_lse[:, :rows])
