@@ -428,7 +428,8 @@ int ca_flash_window(const void* q, const void* k, const void* v, void* out, floa
     return CA_ESHAPE;
   if (window_left < -1 || window_right < -1 || sink_tokens < 0) return CA_ESHAPE;
   if (batch == 0 || (var && total_q == 0)) return CA_OK;
-  if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides) return CA_ENULL;
+  // (packed sequences none of which has a key: k and v have no address, and are not read)
+  if (!q || !out || !q_strides || !k_strides || !v_strides || ((!k || !v) && !(var && total_k == 0))) return CA_ENULL;
   const size_t es = elem_size(dtype);
   if (!aligned(q, es) || !aligned(k, es) || !aligned(v, es) || !aligned(out, es) || !aligned(lse, 4))
     return CA_ELAYOUT;

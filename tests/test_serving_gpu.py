@@ -1242,3 +1242,17 @@ def test_prefill_packed_offsets_past_the_tokens(dtype, window):
                 assert status() == K.STATUS_LENS
                 rows = good[2]
                 assert torch.equal(out[:rows], want[:rows]) and torch.equal(lse[:, :rows], want_lse[:, :rows])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("window", [(-1, -1), (5, 0), (3, 9)])
+def test_prefill_packed_without_any_key(dtype, window):
+    """Packed sequences none of which has a key (the packed k and v are empty): zeros, and log-sum-exps of -inf."""
+    q = torch.randn(9, 4, 64, generator=torch.Generator().manual_seed(0)).to(dtype).to(DEV)
+    kv = torch.zeros(0, 2, 64, dtype=dtype, device=DEV)
+    cq, ck = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 2, 9], [0, 0, 0]))
+    for causal in (False, True):
+        out, lse = api().flash_attn_varlen_func(q, kv, kv, cq, ck, 7, 1, causal=causal, window_size=window, sink_tokens=2,
+                                                return_attn_probs=True)
+        assert out.shape == q.shape and (out == 0).all() and torch.isneginf(lse).all()
+    assert status() == 0
