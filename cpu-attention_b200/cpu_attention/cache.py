@@ -168,8 +168,9 @@ def _explain_append(key, value, k_cache, v_cache, k_scale, v_scale, lens, table,
     if cu is None:
         if key.shape[0] != batch:
             raise ValueError("cpu_attention: key/value and cache_seqlens disagree on the batch")
-        longest = key.shape[1]
-        if batch and longest and int(lens.max()) + longest > table.shape[1] * page:
+        new = key.shape[1]
+        longest = int(lens.max()) if batch and new else -1  # (negative: every sequence is left out)
+        if longest >= 0 and longest + new > table.shape[1] * page:
             raise ValueError("cpu_attention: cache_seqlens exceed the page table's capacity")
     else:
         if not isinstance(cu, torch.Tensor) or cu.dtype != torch.int32 or tuple(cu.shape) != (batch + 1,):

@@ -255,7 +255,8 @@ def _explain_split(q, k_cache, v_cache, k, v, k_scale, v_scale, lens, table):
             new < 0 or tuple(k.shape) != (batch, new, kv_heads, hd) or v.shape != k.shape or k.dtype != q.dtype
             or v.dtype != q.dtype):
         raise ValueError("cpu_attention: k/v must both be [batch, seqlen_new, nheads, headdim]")
-    if batch and int(lens.max()) + new > table.shape[1] * k_cache.shape[2]:
+    longest = int(lens.max()) if batch else -1  # (negative: every sequence is left out)
+    if longest >= 0 and longest + new > table.shape[1] * k_cache.shape[2]:
         raise ValueError("cpu_attention: cache_seqlens exceed the page table's capacity")
     dev = q.device
     data = [k_cache, v_cache] + ([k, v] if k is not None else []) + ([k_scale, v_scale] if eight else [])

@@ -293,3 +293,18 @@ def test_refused_window_names_the_way():
     for caches in ((f, f.clone(), {}), (kc, vc, dict(k_descale=ks, v_descale=vs))):
         with pytest.raises(NotImplementedError, match="sink_tokens=0"):
             C.flash_attn_with_kvcache(q, *caches[:2], cache_seqlens=4, page_table=bt, window_size=(8, 0), **caches[2])
+
+
+def test_negative_lengths_pass_the_capacity_check():
+    """Sequences left out by a negative length have no tokens to place: the call goes on to the device check."""
+    q, kc, vc, bt, ks, vs = eight()
+    k, out = torch.randn(2, 40, 2, 64), torch.tensor([-1, -3], dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        C.flash_attn_with_kvcache(q, kc, vc, k=k, v=k, cache_seqlens=out, page_table=bt, k_descale=ks, v_descale=vs)
+    with pytest.raises(ValueError, match="CUDA"):
+        C.append_quantized(k, k, kc, vc, ks, vs, out, bt)
+    out[0] = 0
+    with pytest.raises(ValueError, match="capacity"):
+        C.flash_attn_with_kvcache(q, kc, vc, k=k, v=k, cache_seqlens=out, page_table=bt, k_descale=ks, v_descale=vs)
+    with pytest.raises(ValueError, match="capacity"):
+        C.append_quantized(k, k, kc, vc, ks, vs, out, bt)
