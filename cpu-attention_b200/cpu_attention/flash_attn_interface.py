@@ -117,8 +117,9 @@ def flash_attn_with_kvcache(
     ``k_descale`` and ``v_descale``, float32 ``[num_blocks, nheads_k]``: a value
     is its code times its block's and head's scale. (flash-attn's arguments of
     these names are ``[batch, nheads_k]``, one scale per sequence; scales laid
-    out so do not belong here, also where the two shapes happen to be equal.) ``q`` (and ``k``/``v``) stay
-    fp32 or bf16; appending updates caches and scales.
+    out so do not belong here, also where the two shapes happen to be equal.)
+    ``q`` (and ``k``/``v``) stay fp32 or bf16; appending updates caches and
+    scales.
 
     ``sink_tokens`` (0 or more) turns ``window_size`` on, for float and 8-bit
     caches: the query, at the last position, sees the last ``window_size[0] +

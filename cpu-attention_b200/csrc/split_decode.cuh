@@ -53,8 +53,8 @@
 //
 // 8-bit and bf16 caches: loads of tile n+1 are issued as soon as the registers of
 // tile n are free: 12 warps an SM with a tile each in flight are 48 KiB, about
-// twice what HBM's latency asks for; 8-bit tiles are called into L2 one tile earlier still (-8%;
-// four tiles earlier: +4%, eight: +17%). Measured against this (8-bit grouped,
+// twice what HBM's latency asks for; 8-bit tiles are called into L2 one tile
+// earlier still (-8%; four tiles earlier: +4%, eight: +17%). Measured against this (8-bit grouped,
 // 96 us then): cp.async into shared memory with four tiles ahead 132 us, TMA
 // tiles swizzled for conflict-free fragment loads 96 us, two tiles ahead in
 // registers 98 us, the next tile's scores before this one's weights 117 us, 8
